@@ -2,7 +2,7 @@
 
 * ``libsvtad_sparse.so``: every ``csrc/*.hip`` compiled by hipcc for gfx950.
   This is the C-ABI library (``include/svtad_sparse.h``).
-* ``opentad_sparse_ops*.so``: the PyTorch extension (``csrc/torch_ext.cpp``,
+* ``opentad_sparse_ops*.so``: the PyTorch extension (``csrc/torch_ext*.cpp``,
   host C++ compiled by g++ against torch's headers), linked to
   ``libsvtad_sparse.so`` with an ``$ORIGIN`` rpath.
 
@@ -77,7 +77,7 @@ def ext_cmd():
            "-D_GLIBCXX_USE_CXX11_ABI=1"]
     for p in inc + [pybind11.get_include(), py_inc, os.path.join(ROCM, "include")]:
         cmd += ["-I", p]
-    cmd += [os.path.join(CSRC, "torch_ext.cpp"), "-o", EXT + ".tmp",
+    cmd += [*sorted(glob.glob(os.path.join(CSRC, "*.cpp"))), "-o", EXT + ".tmp",
             "-L", libdir, "-L", PKG, "-lsvtad_sparse", "-lc10", "-lc10_hip", "-ltorch",
             "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + libdir]
     return cmd

@@ -1,0 +1,158 @@
+// C ABI of cross attention: checks, the split of the work, dispatch by type.
+#include "cross_attn.h"
+
+#include <algorithm>
+#include <cmath>
+
+namespace svtad {
+
+constexpr int kMaxHeadDim = 128;
+constexpr int kWantGroups = 512;  // two workgroups per compute unit
+constexpr int kMaxSplits = 64;
+
+// How a kernel over row tiles (forward, dq) is cut: waves along the rows, and
+// splits of the keys. Rows are not padded to more than twice their number where
+// fewer waves can hold them; the keys are split while there are fewer row
+// tiles than the chip takes at once, into parts of at least two staged tiles.
+struct RowPlan {
+    int wave_rows, splits;
+};
+
+static RowPlan row_plan(const svtad_cross_args& a) {
+    const int64_t m = a.nq * (a.heads / a.kv_heads);
+    RowPlan r{m <= 16 ? 1 : m <= 64 ? 2 : 4, 1};
+    const int64_t rows = r.wave_rows == 4 ? 128 : r.wave_rows == 2 ? 64 : 16;
+    const int64_t groups = std::max<int64_t>(1, cdiv(m, rows) * a.batch * a.kv_heads);
+    const int64_t tiles = cdiv(a.nk, r.wave_rows == 1 ? 128 : 64);
+    r.splits = (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(kWantGroups, groups), tiles / 2, (int64_t)kMaxSplits}));
+    return r;
+}
+
+// Splits of the rows in the kernel over key tiles.
+static int key_plan(const svtad_cross_args& a) {
+    const int64_t m = a.nq * (a.heads / a.kv_heads);
+    const int64_t groups = std::max<int64_t>(1, cdiv(a.nk, cross_kv_keys(a.head_dim)) * a.batch * a.kv_heads);
+    return (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(kWantGroups, groups), cdiv(m, 64) / 2, (int64_t)kMaxSplits}));
+}
+
+static size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+static int64_t all_rows(const svtad_cross_args& a) { return a.batch * a.heads * a.nq; }
+static int64_t pad4(int d) { return (d + 3) & ~3; }
+
+static size_t fwd_bytes(const svtad_cross_args& a) {
+    const int s = row_plan(a).splits;
+    return s > 1 ? (size_t)s * all_rows(a) * (pad4(a.head_dim) + 2) * 4 : 0;
+}
+
+static size_t bwd_bytes(const svtad_cross_args& a) {
+    const int sq = row_plan(a).splits, sk = key_plan(a);
+    const size_t pq = sq > 1 ? (size_t)sq * all_rows(a) * pad4(a.head_dim) * 4 : 0;
+    const size_t pk = sk > 1 ? (size_t)sk * 2 * a.batch * a.kv_heads * a.nk * pad4(a.head_dim) * 4 : 0;
+    return align256((size_t)all_rows(a) * 4) + std::max(pq, pk);
+}
+
+static int cross_check(const svtad_cross_args* a, int dtype) {
+    if (!a) return set_error(SVTAD_ERR_INVALID, "cross_attention: args is NULL");
+    if (dtype != SVTAD_F32 && dtype != SVTAD_F16 && dtype != SVTAD_BF16)
+        return set_error(SVTAD_ERR_INVALID, "cross_attention: dtype must be float32, float16 or bfloat16");
+    if (a->batch < 0 || a->nq < 0 || a->nk < 0) return set_error(SVTAD_ERR_INVALID, "cross_attention: negative size");
+    if (a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads)
+        return set_error(SVTAD_ERR_INVALID, "cross_attention: the query heads must be a multiple of the key heads");
+    if (a->head_dim < 1 || a->head_dim > kMaxHeadDim)
+        return set_error(SVTAD_ERR_UNSUPPORTED, "cross_attention: the head dimension must be 1 to 128");
+    if (!(a->scale > 0.f) || !std::isfinite(a->scale))
+        return set_error(SVTAD_ERR_INVALID, "cross_attention: scale must be positive and finite");
+    const double m = (double)a->nq * (a->heads / a->kv_heads), bk = (double)a->batch * a->kv_heads;
+    if ((m / 16 + 1) * bk * kMaxSplits > INT32_MAX || ((double)a->nk / 64 + 1) * bk * kMaxSplits > INT32_MAX ||
+        bk * std::max(m, (double)a->nk) * 64 > (double)INT32_MAX * 256)
+        return set_error(SVTAD_ERR_UNSUPPORTED, "cross_attention: too many rows or keys for one launch");
+    return SVTAD_OK;
+}
+
+static CrossArgs cross_args(const svtad_cross_args& a) {
+    CrossArgs p{};
+    p.q = a.q, p.k = a.k, p.v = a.v;
+    p.qb = a.q_stride[0], p.qn = a.q_stride[1], p.qh = a.q_stride[2];
+    p.kb = a.k_stride[0], p.kn = a.k_stride[1], p.kh = a.k_stride[2];
+    p.vb = a.v_stride[0], p.vn = a.v_stride[1], p.vh = a.v_stride[2];
+    p.lengths = a.lengths;
+    p.mask = a.mask, p.mask_b = a.mask_stride[0], p.mask_n = a.mask_stride[1];
+    p.B = (int)a.batch, p.H = a.heads, p.KH = a.kv_heads, p.G = a.heads / a.kv_heads, p.D = a.head_dim;
+    p.Nq = a.nq, p.Nk = a.nk, p.M = a.nq * p.G;
+    p.scale = a.scale;
+    p.c = (float)((double)a.scale * 1.4426950408889634);
+    p.splits = 1;
+    return p;
+}
+
+}  // namespace svtad
+
+using namespace svtad;
+
+extern "C" size_t svtad_cross_attention_workspace_bytes(const svtad_cross_args* a, int dtype) {
+    return cross_check(a, dtype) ? 0 : fwd_bytes(*a);
+}
+
+extern "C" size_t svtad_cross_attention_bwd_workspace_bytes(const svtad_cross_args* a, int dtype) {
+    return cross_check(a, dtype) ? 0 : bwd_bytes(*a);
+}
+
+extern "C" int svtad_cross_attention(const svtad_cross_args* a, void* out, float* lse, void* workspace,
+                                     size_t workspace_bytes, int dtype, void* stream) {
+    const int st = cross_check(a, dtype);
+    if (st) return st;
+    if (all_rows(*a) == 0) return SVTAD_OK;
+    if (!a->q || !out || (a->nk > 0 && (!a->k || !a->v))) return set_error(SVTAD_ERR_INVALID, "cross_attention: NULL pointer");
+    const size_t need = fwd_bytes(*a);
+    if (need && (!workspace || workspace_bytes < need))
+        return set_error(SVTAD_ERR_WORKSPACE, "cross_attention: workspace too small");
+    const RowPlan plan = row_plan(*a);
+    CrossArgs p = cross_args(*a);
+    p.out = out, p.lse = lse;
+    p.splits = plan.splits, p.part = (float*)workspace;
+    if (dtype == SVTAD_F16) cross_fwd<f16>(p, plan.wave_rows, (hipStream_t)stream);
+    else if (dtype == SVTAD_BF16) cross_fwd<bf16>(p, plan.wave_rows, (hipStream_t)stream);
+    else cross_fwd<float>(p, plan.wave_rows, (hipStream_t)stream);
+    return launch_status();
+}
+
+template <typename T>
+static void cross_bwd(CrossArgs p, const svtad_cross_args& a, hipStream_t st) {
+    const RowPlan plan = row_plan(a);
+    float* const part = p.part;
+    if (p.M > 0) {
+        p.splits = p.out ? plan.splits : 1;
+        cross_bwd_q<T>(p, plan.wave_rows, st);
+    }
+    if (p.dk && a.nk > 0) {
+        p.splits = key_plan(a), p.part = part;
+        cross_bwd_kv<T>(p, st);
+    }
+}
+
+extern "C" int svtad_cross_attention_bwd(const svtad_cross_args* a, const void* out, const float* lse, const void* dout,
+                                         const int64_t* dout_stride, void* dq, void* dk, void* dv, void* workspace,
+                                         size_t workspace_bytes, int dtype, void* stream) {
+    const int st = cross_check(a, dtype);
+    if (st) return st;
+    if (!dk != !dv) return set_error(SVTAD_ERR_INVALID, "cross_attention_bwd: dk and dv come together");
+    if ((!dq && !dk) || a->batch == 0) return SVTAD_OK;
+    if (a->nq > 0 && (!a->q || !out || !lse || !dout || !dout_stride || (a->nk > 0 && (!a->k || !a->v))))
+        return set_error(SVTAD_ERR_INVALID, "cross_attention_bwd: NULL pointer");
+    const size_t need = bwd_bytes(*a);
+    if (need && (!workspace || workspace_bytes < need))
+        return set_error(SVTAD_ERR_WORKSPACE, "cross_attention_bwd: workspace too small");
+    CrossArgs p = cross_args(*a);
+    p.o = out, p.on = (int64_t)a->heads * a->head_dim, p.oh = a->head_dim, p.ob = a->nq * p.on;
+    p.dout = dout;
+    if (dout_stride) p.gb = dout_stride[0], p.gn = dout_stride[1], p.gh = dout_stride[2];
+    p.out = dq, p.dk = dk, p.dv = dv;
+    p.lse = const_cast<float*>(lse);
+    p.delta = (float*)workspace;
+    p.part = (float*)((char*)workspace + align256((size_t)all_rows(*a) * 4));
+    hipStream_t hs = (hipStream_t)stream;
+    if (dtype == SVTAD_F16) cross_bwd<f16>(p, *a, hs);
+    else if (dtype == SVTAD_BF16) cross_bwd<bf16>(p, *a, hs);
+    else cross_bwd<float>(p, *a, hs);
+    return launch_status();
+}

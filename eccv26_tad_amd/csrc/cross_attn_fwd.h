@@ -1,0 +1,296 @@
+// Cross attention, forward: kernels and launch.
+//
+//   s = scale q . k,  p = softmax of s over the seen keys,  out = sum p v
+//
+// One pass over the keys with each row's running maximum and sum (float32).
+// A workgroup of 4 waves owns WM R 16 rows of one key head (R row tiles of 16
+// per wave) and walks over key tiles staged in LDS, the next tile's loads in
+// flight in registers meanwhile; with WM < 4 the waves of equal rows share a
+// tile's keys and are joined at the end. Rows are queries times the G query
+// heads of the key head, so shared key heads are read once for all of them.
+// With few rows the keys are split over workgroups, whose partial sums
+// k_cross_join adds in a fixed order.
+//
+// Probabilities are rounded to T for the product with v (the matrix units'
+// operand type); their sum, the maximum and the output's sums stay float32.
+// Keys that are not seen are staged as zeros and their scores replaced, so
+// neither infinities nor NaN in their places reach a result.
+#pragma once
+
+#include "cross_attn.h"
+
+namespace svtad {
+
+constexpr float kNegInf = -__builtin_huge_valf();
+
+// Keys of a staged tile: 64, or 32 per wave where the waves share a tile.
+template <int WM> constexpr int kTileKeys = WM == 1 ? 128 : 64;
+
+// One thread's share of a tile of TILE rows by W elements: loads to registers
+// and stores to LDS. Rows for which `row` gives NULL are zeros.
+template <typename T, int TILE, int W>
+struct Stage {
+    static constexpr int kChunks = TILE * W / 8 / 256;
+    Frag8<T> v[kChunks];
+
+    template <typename F>
+    __device__ __forceinline__ void load(F row, int d) {
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) {
+            const int ch = threadIdx.x + i * 256, r = ch / (W / 8), c = ch % (W / 8) * 8;
+            const T* const at = row(r);
+            v[i] = at ? load_frag<T>(at, c, d) : zero_frag<T>();
+        }
+    }
+    __device__ __forceinline__ void store(T* lds) const {
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) {
+            const int ch = threadIdx.x + i * 256, r = ch / (W / 8), c = ch % (W / 8) * 8;
+            *(Frag8<T>*)(lds + r * kPitch<T, W> + c) = v[i];
+        }
+    }
+};
+
+template <typename T, int DP, int WM, int R>
+__global__ __launch_bounds__(256) void k_cross_fwd(CrossArgs p) {
+    constexpr int W = DP < 32 ? 32 : DP, KS = W / 32, DB = DP / 16, P = kPitch<T, W>;
+    constexpr int WK = 4 / WM, TK = kTileKeys<WM>, KW = TK / WK, NB = KW / 16, ROWS = WM * R * 16;
+    static_assert(KW % 32 == 0, "a wave's keys fill whole products");
+    constexpr size_t kTiles = 2 * (size_t)TK * P * sizeof(T), kJoin = WK > 1 ? (size_t)WK * ROWS * (DP + 2) * 4 : 0;
+    __shared__ __attribute__((aligned(16))) unsigned char mem[kTiles > kJoin ? kTiles : kJoin];
+    __shared__ __attribute__((aligned(16))) uint8_t seen[TK];
+    T* const lk = (T*)mem;
+    T* const lv = lk + TK * P;
+
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave % WM, wk = wave / WM;
+    const int g = lane >> 4, li = lane & 15;
+    const int64_t row_tiles = cdiv(p.M, ROWS);
+    int64_t t = xcd_tile(blockIdx.x, gridDim.x);
+    const int64_t r0 = t % row_tiles * ROWS;
+    t /= row_tiles;
+    const int split = (int)(t % p.splits);
+    const int bh = (int)(t / p.splits), b = bh / p.KH, j = bh - b * p.KH;
+    const int64_t len = seen_length(p, b);
+    const int64_t tiles = cdiv(len, TK), per = cdiv(tiles, p.splits);
+    const int64_t t0 = split * per, t1 = min(tiles, t0 + per);
+
+    Frag8<T> qf[R][KS];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int64_t r = r0 + (wm * R + i) * 16 + li;
+        const T* const q = (const T*)p.q + b * p.qb + (r < p.M ? row_at(p, r, p.qn, p.qh, j) : 0);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) qf[i][s] = r < p.M ? load_frag<T>(q, s * 32 + g * 8, p.D) : zero_frag<T>();
+    }
+
+    const T* const kbase = (const T*)p.k + b * p.kb + j * p.kh;
+    const T* const vbase = (const T*)p.v + b * p.vb + j * p.vh;
+    const uint8_t* const mbase = p.mask ? p.mask + b * p.mask_b : nullptr;
+    auto is_seen = [&](int64_t key) { return key < len && (!mbase || mbase[key * p.mask_n]); };
+    Stage<T, TK, W> sk, sv;
+    bool ms = false;
+    auto fetch = [&](int64_t tile) {
+        sk.load([&](int r) { const int64_t key = tile * TK + r; return is_seen(key) ? kbase + key * p.kn : nullptr; }, p.D);
+        sv.load([&](int r) { const int64_t key = tile * TK + r; return is_seen(key) ? vbase + key * p.vn : nullptr; }, p.D);
+        if (mbase && threadIdx.x < TK) ms = is_seen(tile * TK + threadIdx.x);
+    };
+
+    f32x4 acc[DB][R];
+    float m[R], l[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        m[i] = kNegInf, l[i] = 0.f;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) acc[db][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    if (t0 < t1) fetch(t0);
+    for (int64_t tile = t0; tile < t1; ++tile) {
+        __syncthreads();
+        sk.store(lk);
+        sv.store(lv);
+        if (mbase && threadIdx.x < TK) seen[threadIdx.x] = ms;
+        __syncthreads();
+        if (tile + 1 < t1) fetch(tile + 1);
+
+        f32x4 s[NB][R];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+            for (int i = 0; i < R; ++i) s[nb][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const Frag8<T> a = lds_frag<T>(lk + (wk * KW + nb * 16 + li) * P + ks * 32 + g * 8);
+#pragma unroll
+                for (int i = 0; i < R; ++i) s[nb][i] = mma<T>(a, qf[i][ks], s[nb][i]);
+            }
+        }
+        if (mbase) {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                const uint32_t w = *(const uint32_t*)(seen + wk * KW + nb * 16 + 4 * g);
+#pragma unroll
+                for (int i = 0; i < R; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[nb][i][e] = (w >> (8 * e)) & 0xff ? s[nb][i][e] : kNegInf;
+            }
+        } else if ((tile + 1) * TK > len) {
+            const int left = (int)(len - tile * TK) - wk * KW - 4 * g;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int i = 0; i < R; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[nb][i][e] = nb * 16 + e < left ? s[nb][i][e] : kNegInf;
+        }
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            float mx = s[0][i][0];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[nb][i][e]);
+            mx = fmaxf(across_groups_max(mx), m[i]);
+            if (__any(mx > m[i])) {  // else the sums keep their scale
+                const float f = mx == kNegInf ? 1.f : __builtin_amdgcn_exp2f((m[i] - mx) * p.c);
+                m[i] = mx;
+                l[i] *= f;
+#pragma unroll
+                for (int db = 0; db < DB; ++db) acc[db][i] *= f;
+            }
+            const float mc = mx == kNegInf ? 0.f : mx * p.c;  // no key seen so far: every power is 0
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[nb][i][e] = __builtin_amdgcn_exp2f(fmaf(s[nb][i][e], p.c, -mc));
+                    l[i] += s[nb][i][e];
+                }
+        }
+#pragma unroll
+        for (int kg = 0; kg < NB / 2; ++kg) {
+            Frag8<T> pf[R];
+#pragma unroll
+            for (int i = 0; i < R; ++i) pf[i] = pack_frag<T>(s[2 * kg][i], s[2 * kg + 1][i]);
+#pragma unroll
+            for (int db = 0; db < DB; ++db) {
+                const Frag8<T> a = lds_frag_t<T, P>(lv + (wk * KW + kg * 32) * P, db * 16, lane);
+#pragma unroll
+                for (int i = 0; i < R; ++i) acc[db][i] = mma<T>(a, pf[i], acc[db][i]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) l[i] = across_groups_sum(l[i]);
+
+    if constexpr (WK > 1) {  // join the waves of equal rows, in order
+        float* const jo = (float*)mem;               // [WK][ROWS][DP]
+        float* const jm = jo + WK * ROWS * DP;       // [WK][ROWS][2]
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int r = (wm * R + i) * 16 + li;
+            if (g == 0) {
+                jm[(wk * ROWS + r) * 2] = m[i];
+                jm[(wk * ROWS + r) * 2 + 1] = l[i];
+            }
+#pragma unroll
+            for (int db = 0; db < DB; ++db) *(f32x4*)(jo + (wk * ROWS + r) * DP + db * 16 + 4 * g) = acc[db][i];
+        }
+        __syncthreads();
+        if (wk != 0) return;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int r = (wm * R + i) * 16 + li;
+            float top = m[i];
+#pragma unroll
+            for (int w = 1; w < WK; ++w) top = fmaxf(top, jm[(w * ROWS + r) * 2]);
+            if (top == kNegInf) continue;
+            float f = __builtin_amdgcn_exp2f((m[i] - top) * p.c);
+            l[i] *= f;
+#pragma unroll
+            for (int db = 0; db < DB; ++db) acc[db][i] *= f;
+#pragma unroll
+            for (int w = 1; w < WK; ++w) {
+                f = __builtin_amdgcn_exp2f((jm[(w * ROWS + r) * 2] - top) * p.c);
+                l[i] += f * jm[(w * ROWS + r) * 2 + 1];
+#pragma unroll
+                for (int db = 0; db < DB; ++db) acc[db][i] += *(const f32x4*)(jo + (w * ROWS + r) * DP + db * 16 + 4 * g) * f;
+            }
+            m[i] = top;
+        }
+    }
+
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int64_t r = r0 + (wm * R + i) * 16 + li;
+        if (r >= p.M) continue;
+        if (p.splits > 1) {
+            const int64_t at = ((int64_t)split * p.B * p.KH + bh) * p.M + r;
+            const int dp = (p.D + 3) & ~3;
+            float* const po = p.part + at * dp;
+            float* const pm = p.part + (int64_t)p.splits * p.B * p.KH * p.M * dp + at * 2;
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+                if (db * 16 + 4 * g < p.D) *(f32x4*)(po + db * 16 + 4 * g) = acc[db][i];
+            if (g == 0) {
+                pm[0] = m[i];
+                pm[1] = l[i];
+            }
+            continue;
+        }
+        T* const o = (T*)p.out + (int64_t)b * p.Nq * p.H * p.D + row_at(p, r, (int64_t)p.H * p.D, p.D, j);
+        const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
+#pragma unroll
+        for (int db = 0; db < DB; ++db) store4<T>(o, db * 16 + 4 * g, p.D, acc[db][i] * inv);
+        if (p.lse && g == 0)
+            p.lse[bh * p.M + r] = l[i] == 0.f ? -kNegInf : m[i] * p.c + __builtin_amdgcn_logf(l[i]);
+    }
+}
+
+// The splits of a row joined in order: one thread per 4 output values.
+template <typename T>
+__global__ __launch_bounds__(256) void k_cross_join(CrossArgs p) {
+    const int dp = (p.D + 3) & ~3, nd = dp / 4;
+    const int64_t rows = (int64_t)p.B * p.KH * p.M, e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (e >= rows * nd) return;
+    const int64_t at = e / nd;
+    const int c = (int)(e - at * nd) * 4;
+    const float* const pm = p.part + (int64_t)p.splits * rows * dp;
+    float top = kNegInf;
+    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, pm[(s * rows + at) * 2]);
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    float l = 0.f;
+    if (top != kNegInf)
+        for (int s = 0; s < p.splits; ++s) {
+            const float f = __builtin_amdgcn_exp2f((pm[(s * rows + at) * 2] - top) * p.c);
+            l += f * pm[(s * rows + at) * 2 + 1];
+            acc += *(const f32x4*)(p.part + (s * rows + at) * dp + c) * f;
+        }
+    const int64_t bh = at / p.M, r = at - bh * p.M, b = bh / p.KH;
+    const int j = (int)(bh - b * p.KH);
+    T* const o = (T*)p.out + b * p.Nq * p.H * p.D + row_at(p, r, (int64_t)p.H * p.D, p.D, j);
+    store4<T>(o, c, p.D, acc * (l == 0.f ? 0.f : 1.f / l));
+    if (p.lse && c == 0) p.lse[at] = l == 0.f ? -kNegInf : top * p.c + __builtin_amdgcn_logf(l);
+}
+
+template <typename T, int WM, int R>
+static void launch_cross_fwd(const CrossArgs& p, hipStream_t st) {
+    const int64_t grid = cdiv(p.M, WM * R * 16) * p.B * p.KH * p.splits;
+    if (p.D <= 16) k_cross_fwd<T, 16, WM, R><<<(unsigned)grid, 256, 0, st>>>(p);
+    else if (p.D <= 32) k_cross_fwd<T, 32, WM, R><<<(unsigned)grid, 256, 0, st>>>(p);
+    else if (p.D <= 64) k_cross_fwd<T, 64, WM, R><<<(unsigned)grid, 256, 0, st>>>(p);
+    else k_cross_fwd<T, 128, WM, R><<<(unsigned)grid, 256, 0, st>>>(p);
+}
+
+template <typename T>
+void cross_fwd(const CrossArgs& p, int wave_rows, hipStream_t st) {
+    if (wave_rows == 4) launch_cross_fwd<T, 4, 2>(p, st);
+    else if (wave_rows == 2) launch_cross_fwd<T, 2, 2>(p, st);
+    else launch_cross_fwd<T, 1, 1>(p, st);
+    if (p.splits > 1) {
+        const int64_t n = (int64_t)p.B * p.KH * p.M * ((p.D + 3) / 4);
+        k_cross_join<T><<<(unsigned)cdiv(n, 256), 256, 0, st>>>(p);
+    }
+}
+
+}  // namespace svtad

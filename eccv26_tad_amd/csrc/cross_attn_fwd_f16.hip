@@ -1,0 +1,6 @@
+// Cross attention, forward, for float16 (cross_attn_fwd.h).
+#include "cross_attn_fwd.h"
+
+namespace svtad {
+template void cross_fwd<f16>(const CrossArgs&, int, hipStream_t);
+}  // namespace svtad

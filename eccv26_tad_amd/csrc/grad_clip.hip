@@ -1,0 +1,288 @@
+// The norm over all gradients of a model, and the gradients scaled down to a
+// limit (gfx950).
+//
+//   n = (sum over tensors and elements of g^2)^(1/2)   or   max |g|
+//   out = g scale min(1, limit / (n |scale| + 1e-6))
+//
+// Two passes over many tensors, each launch over up to kTensors of them whose
+// addresses travel in the kernel's arguments: no table in memory, no copy, and
+// a captured graph replays it. The elements of a launch's tensors, laid end to
+// end, are cut into one equal range per workgroup, which finds its first
+// tensor by bisection and walks on from there, so that a model's many small
+// tensors cost no workgroup of their own.
+//
+// Squares are summed in float64: float32 gradients neither overflow nor lose
+// small addends, at a rate the vector units outrun memory at (bound by its
+// bytes). Every workgroup leaves one partial sum; the scaling pass adds them
+// in one fixed order in each of its workgroups, without a launch between.
+#include <algorithm>
+
+#include "sv_internal.h"
+#include "sv_vec.h"
+
+namespace svtad {
+
+constexpr int kTensors = 160;  // of a launch: 24 bytes each of the 4 KB of kernel arguments
+constexpr int kMaxGroups = 1024;
+constexpr double kClipEps = 1e-6;
+
+struct ClipList {
+    const void* g[kTensors];
+    void* out[kTensors];
+    int64_t end[kTensors];  // elements of the tensors up to and with this one
+    int count, g_type, out_type;
+};
+static_assert(sizeof(ClipList) + 64 <= 4096, "kernel arguments");
+
+struct ClipScale {
+    const double* part;
+    float* norm;         // written by one workgroup of one launch (NULL: not by this one)
+    int parts;
+    float limit, scale;  // limit < 0: no clipping
+    bool inf;
+};
+
+// First tensor whose end is past element e
+__device__ __forceinline__ int clip_find(const ClipList& t, int64_t e) {
+    int lo = 0, hi = t.count - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (t.end[mid] > e) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
+}
+
+template <bool INF>
+__device__ __forceinline__ double clip_join(double a, double b) {
+    if constexpr (INF) return (b > a || b != b) ? b : a;  // a NaN stays
+    else return a + b;
+}
+
+// Over the workgroup's 256 threads, in a fixed order, in every thread
+template <bool INF>
+__device__ __forceinline__ double clip_reduce(double v) {
+    __shared__ double red[4];
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) v = clip_join<INF>(v, __shfl_xor(v, m, 64));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return clip_join<INF>(clip_join<INF>(red[0], red[1]), clip_join<INF>(red[2], red[3]));
+}
+
+constexpr int kUnroll = 4;  // 16-byte loads in flight per thread
+
+template <typename T, bool INF>
+__global__ __launch_bounds__(256) void k_grad_norm(ClipList t, double* part) {
+    constexpr int V = kVec<T>;
+    const int64_t total = t.end[t.count - 1];
+    const int64_t per = cdiv(cdiv(total, gridDim.x), 64) * 64;
+    int64_t e = (int64_t)blockIdx.x * per;
+    const int64_t e1 = min(total, e + per);
+    double acc = 0.0;
+    auto add = [&](T v) {
+        const double d = (double)(float)v;
+        acc = INF ? clip_join<true>(acc, fabs(d)) : fma(d, d, acc);
+    };
+    for (int i = e < e1 ? clip_find(t, e) : 0; e < e1; ++i) {
+        const int64_t first = i ? t.end[i - 1] : 0, stop = min(e1, t.end[i]);
+        const T* const g = (const T*)t.g[i] + (e - first);
+        const int64_t n = stop - e, body = n / (256 * V) * (256 * V);
+        int64_t at = threadIdx.x * V;
+        for (; at + (kUnroll - 1) * 256 * V < body; at += kUnroll * 256 * V) {
+            Pack<T, V> v[kUnroll];
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) v[u] = *(const Pack<T, V>*)(g + at + u * 256 * V);
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+                for (int k = 0; k < V; ++k) add(v[u].e[k]);
+        }
+        for (; at < body; at += 256 * V) {
+            const Pack<T, V> v = *(const Pack<T, V>*)(g + at);
+#pragma unroll
+            for (int k = 0; k < V; ++k) add(v.e[k]);
+        }
+        for (int64_t q = body + threadIdx.x; q < n; q += 256) add(g[q]);
+        e = stop;
+    }
+    acc = clip_reduce<INF>(acc);
+    if (threadIdx.x == 0) part[blockIdx.x] = acc;
+}
+
+// The norm of all partial sums (before scale), in every thread
+__device__ __forceinline__ double clip_norm(const ClipScale& s) {
+    double a = 0.0;
+    if (s.inf) {
+        for (int i = threadIdx.x; i < s.parts; i += 256) a = clip_join<true>(a, s.part[i]);
+        return clip_reduce<true>(a);
+    }
+    for (int i = threadIdx.x; i < s.parts; i += 256) a += s.part[i];
+    return sqrt(clip_reduce<false>(a));
+}
+
+__global__ __launch_bounds__(256) void k_grad_norm_out(ClipScale s) {
+    const double n = clip_norm(s) * fabs((double)s.scale);
+    if (threadIdx.x == 0) *s.norm = (float)n;
+}
+
+// Ranges in the opposite order: what the norm's pass read last is in the cache
+// still.
+template <typename T, typename O>
+__global__ __launch_bounds__(256) void k_grad_scale(ClipList t, ClipScale s) {
+    constexpr int V = kVec<T>;
+    const double n = clip_norm(s) * fabs((double)s.scale);
+    if (s.norm && blockIdx.x == 0 && threadIdx.x == 0) *s.norm = (float)n;
+    double c = s.limit < 0.f ? 1.0 : (double)s.limit / (n + kClipEps);
+    c = (c > 1.0 ? 1.0 : c) * (double)s.scale;
+    const float f = (float)c;
+    // in place and under the limit: every element keeps its value
+    if (f == 1.f && sizeof(T) == sizeof(O) && t.g[0] == t.out[0]) return;
+    const int64_t total = t.end[t.count - 1];
+    const int64_t per = cdiv(cdiv(total, gridDim.x), 64) * 64;
+    int64_t e = (int64_t)(gridDim.x - 1 - blockIdx.x) * per;
+    const int64_t e1 = min(total, e + per);
+    for (int i = e < e1 ? clip_find(t, e) : 0; e < e1; ++i) {
+        const int64_t first = i ? t.end[i - 1] : 0, stop = min(e1, t.end[i]);
+        const T* const g = (const T*)t.g[i] + (e - first);
+        O* const o = (O*)t.out[i] + (e - first);
+        const int64_t m = stop - e, body = m / (256 * V) * (256 * V);
+        int64_t at = threadIdx.x * V;
+        for (; at + (kUnroll - 1) * 256 * V < body; at += kUnroll * 256 * V) {
+            Pack<T, V> v[kUnroll];
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) v[u] = *(const Pack<T, V>*)(g + at + u * 256 * V);
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+                Pack<O, V> w;
+#pragma unroll
+                for (int k = 0; k < V; ++k) w.e[k] = (O)((float)v[u].e[k] * f);
+                *(Pack<O, V>*)(o + at + u * 256 * V) = w;
+            }
+        }
+        for (; at < body; at += 256 * V) {
+            const Pack<T, V> v = *(const Pack<T, V>*)(g + at);
+            Pack<O, V> w;
+#pragma unroll
+            for (int k = 0; k < V; ++k) w.e[k] = (O)((float)v.e[k] * f);
+            *(Pack<O, V>*)(o + at) = w;
+        }
+        for (int64_t q = body + threadIdx.x; q < m; q += 256) o[q] = (O)((float)g[q] * f);
+        e = stop;
+    }
+}
+
+// Workgroups for `total` elements: one for every 16 KB or so, at most four per
+// compute unit.
+static int clip_groups(int64_t total) {
+    return (int)std::max<int64_t>(1, std::min<int64_t>(cdiv(total, 4096), kMaxGroups));
+}
+
+struct ClipPlan {  // the launches of a list of tensors of any length
+    const svtad_grad* t;
+    int64_t count;
+
+    // The tensors from `at` on that one launch takes: one pair of types, none
+    // empty. Returns the next tensor's number.
+    int64_t take(int64_t at, ClipList& l) const {
+        l.count = 0;
+        int64_t total = 0;
+        for (; at < count && l.count < kTensors; ++at) {
+            const svtad_grad& q = t[at];
+            if (q.count == 0) continue;
+            if (l.count == 0) l.g_type = q.g_type, l.out_type = q.out_type;
+            else if (l.g_type != q.g_type || l.out_type != q.out_type || (l.g[0] == l.out[0]) != (q.g == q.out)) break;
+            l.g[l.count] = q.g, l.out[l.count] = q.out;
+            total += q.count;
+            l.end[l.count++] = total;
+        }
+        return at;
+    }
+
+    int64_t parts() const {
+        ClipList l;
+        int64_t n = 0;
+        for (int64_t at = 0; at < count;) {
+            at = take(at, l);
+            if (l.count) n += clip_groups(l.end[l.count - 1]);
+        }
+        return n;
+    }
+};
+
+template <typename T>
+static void launch_norm(const ClipList& l, bool inf, int grid, double* part, hipStream_t st) {
+    if (inf) k_grad_norm<T, true><<<grid, 256, 0, st>>>(l, part);
+    else k_grad_norm<T, false><<<grid, 256, 0, st>>>(l, part);
+}
+
+template <typename T>
+static void launch_scale(const ClipList& l, const ClipScale& s, int grid, hipStream_t st) {
+    if (l.out_type == SVTAD_F32) k_grad_scale<T, float><<<grid, 256, 0, st>>>(l, s);
+    else if (l.out_type == SVTAD_F16) k_grad_scale<T, f16><<<grid, 256, 0, st>>>(l, s);
+    else k_grad_scale<T, bf16><<<grid, 256, 0, st>>>(l, s);
+}
+
+static int clip_check(const svtad_grad* t, int64_t count, bool with_out) {
+    if (count < 0 || (count > 0 && !t)) return set_error(SVTAD_ERR_INVALID, "grad_clip: bad tensor list");
+    auto ok = [](int d) { return d == SVTAD_F32 || d == SVTAD_F16 || d == SVTAD_BF16; };
+    for (int64_t i = 0; i < count; ++i) {
+        if (!ok(t[i].g_type) || (with_out && !ok(t[i].out_type)))
+            return set_error(SVTAD_ERR_INVALID, "grad_clip: tensors must be float32, float16 or bfloat16");
+        if (t[i].count < 0) return set_error(SVTAD_ERR_INVALID, "grad_clip: negative element count");
+        if (t[i].count > 0 && (!t[i].g || (with_out && !t[i].out))) return set_error(SVTAD_ERR_INVALID, "grad_clip: NULL pointer");
+    }
+    return SVTAD_OK;
+}
+
+}  // namespace svtad
+
+using namespace svtad;
+
+extern "C" size_t svtad_grad_clip_workspace_bytes(const svtad_grad* tensors, int64_t count) {
+    if (!tensors || count < 1) return 0;
+    return (size_t)ClipPlan{tensors, count}.parts() * sizeof(double);
+}
+
+extern "C" int svtad_grad_clip(const svtad_grad* tensors, int64_t count, int norm_type, float max_norm, float scale,
+                               int write, float* norm, void* workspace, size_t workspace_bytes, void* stream) {
+    const int st = clip_check(tensors, count, write != 0);
+    if (st) return st;
+    if (norm_type != SVTAD_NORM_2 && norm_type != SVTAD_NORM_INF)
+        return set_error(SVTAD_ERR_INVALID, "grad_clip: norm_type must be the 2-norm or the maximum");
+    if (!norm) return set_error(SVTAD_ERR_INVALID, "grad_clip: NULL pointer");
+    const ClipPlan plan{tensors, count};
+    const int64_t parts = plan.parts();
+    if (parts > INT32_MAX) return set_error(SVTAD_ERR_UNSUPPORTED, "grad_clip: too many tensors");
+    if (parts > 0 && (!workspace || workspace_bytes < (size_t)parts * sizeof(double)))
+        return set_error(SVTAD_ERR_WORKSPACE, "grad_clip: workspace too small");
+    hipStream_t hs = (hipStream_t)stream;
+    double* const part = (double*)workspace;
+    const bool inf = norm_type == SVTAD_NORM_INF;
+    ClipList l;
+    int64_t done = 0;
+    for (int64_t at = 0; at < count;) {
+        at = plan.take(at, l);
+        if (!l.count) continue;
+        const int grid = clip_groups(l.end[l.count - 1]);
+        if (l.g_type == SVTAD_F32) launch_norm<float>(l, inf, grid, part + done, hs);
+        else if (l.g_type == SVTAD_F16) launch_norm<f16>(l, inf, grid, part + done, hs);
+        else launch_norm<bf16>(l, inf, grid, part + done, hs);
+        done += grid;
+    }
+    ClipScale s{part, norm, (int)parts, max_norm, scale, inf};
+    if (!write || parts == 0) {
+        k_grad_norm_out<<<1, 256, 0, hs>>>(s);
+        return launch_status();
+    }
+    for (int64_t at = 0; at < count;) {
+        at = plan.take(at, l);
+        if (!l.count) continue;
+        const int grid = clip_groups(l.end[l.count - 1]);
+        if (l.g_type == SVTAD_F32) launch_scale<float>(l, s, grid, hs);
+        else if (l.g_type == SVTAD_F16) launch_scale<f16>(l, s, grid, hs);
+        else launch_scale<bf16>(l, s, grid, hs);
+        s.norm = nullptr;
+    }
+    return launch_status();
+}

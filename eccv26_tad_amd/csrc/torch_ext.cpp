@@ -5,39 +5,11 @@
 // The five reference functions keep their names, argument order and meaning
 // (opentad/models/bricks/2d_sparse_v3_bind.cpp:8-14); the rest are additions
 // the autograd wrapper and the table utilities use.
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
-#include <torch/extension.h>
-
 #include <tuple>
 
-#include "../../include/svtad_sparse.h"
+#include "torch_ext.h"
 
 namespace {
-
-int dtype_code(const at::Tensor& t) {
-    switch (t.scalar_type()) {
-        case at::kFloat: return SVTAD_F32;
-        case at::kHalf: return SVTAD_F16;
-        case at::kBFloat16: return SVTAD_BF16;
-        case at::kDouble: return SVTAD_F64;
-        default: TORCH_CHECK(false, "opentad_sparse_ops: unsupported dtype ", t.scalar_type());
-    }
-    return -1;
-}
-
-void* stream_of(const at::Tensor& t) {
-    return (void*)c10::hip::getCurrentHIPStream(t.device().index()).stream();
-}
-
-void check_status(int st, const char* who) {
-    TORCH_CHECK(st == SVTAD_OK, "opentad_sparse_ops.", who, ": ", svtad_last_error(), " (status ",
-                st, ")");
-}
-
-void check_gpu(const at::Tensor& t, const char* name) {
-    TORCH_CHECK(t.is_cuda(), "opentad_sparse_ops: ", name, " must be a GPU tensor");
-}
 
 at::Tensor rows_view(const at::Tensor& t) {
     TORCH_CHECK(t.dim() >= 1, "expected at least 1 dimension");
@@ -1731,5 +1703,6 @@ PYBIND11_MODULE(opentad_sparse_ops, m) {
           py::arg("w"), py::arg("g"), py::arg("b"), py::arg("gs"), py::arg("gamma"));
     m.def("gamma_grad", &op_gamma_grad, "sum(w * g) + sum(b * gs) in fp32 (the adapter's gamma gradient)",
           py::arg("w"), py::arg("g"), py::arg("b"), py::arg("gs"));
+    bind_operators(m);
     m.def("version", []() { return std::string(svtad_version()); });
 }

@@ -1,0 +1,302 @@
+// The extension's transformer operators: layer norm, cross attention, gradient
+// clipping. Checks, outputs and workspaces through the caching allocator, and
+// the current stream of the input's device.
+#include <tuple>
+#include <vector>
+
+#include "torch_ext.h"
+
+namespace {
+
+void check_float(const at::Tensor& t, const char* name) {
+    check_gpu(t, name);
+    const auto st = t.scalar_type();
+    TORCH_CHECK(st == at::kFloat || st == at::kHalf || st == at::kBFloat16, "opentad_sparse_ops: ", name,
+                " must be float32, float16 or bfloat16, got ", st);
+}
+
+at::Tensor workspace(size_t bytes, const at::Tensor& like) {
+    return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : at::Tensor();
+}
+
+void* ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+void* ptr(const c10::optional<at::Tensor>& t) { return t.has_value() ? ptr(*t) : nullptr; }
+
+int64_t row_count(const at::Tensor& t) { return t.size(-1) == 0 ? 0 : t.numel() / t.size(-1); }
+
+// The rows of t [..., c] as at most three axes with strides, c's stride 1; a
+// tensor whose axes do not collapse that far, or whose last axis is strided, is
+// copied.
+struct Rows {
+    at::Tensor t;
+    int64_t d[3], s[3];
+};
+
+Rows rows_of(const at::Tensor& t_in) {
+    Rows r{t_in, {1, 1, 1}, {0, 0, 0}};
+    for (int pass = 0; pass < 2; ++pass) {
+        const at::Tensor& t = r.t;
+        std::vector<int64_t> d, s;  // innermost first
+        if (t.size(-1) <= 1 || t.stride(-1) == 1) {
+            for (int64_t i = t.dim() - 2; i >= 0; --i) {
+                if (t.size(i) == 1) continue;
+                if (!d.empty() && t.stride(i) == d.back() * s.back()) d.back() *= t.size(i);
+                else d.push_back(t.size(i)), s.push_back(t.stride(i));
+            }
+            const int64_t rows = row_count(t);
+            if (d.size() <= 1 || (d.size() <= 3 && rows < ((int64_t)1 << 32))) {
+                // one axis goes first, its neighbours with size 1
+                for (size_t i = 0; i < d.size(); ++i) {
+                    const size_t at = d.size() == 1 ? 0 : 2 - i;
+                    r.d[at] = d[i], r.s[at] = s[i];
+                }
+                return r;
+            }
+        }
+        r.t = t.contiguous();
+    }
+    TORCH_CHECK(false, "opentad_sparse_ops: rows of ", t_in.sizes(), " cannot be walked");
+}
+
+struct NormCall {
+    svtad_norm_args a{};
+    Rows x;
+    at::Tensor w, b;
+};
+
+NormCall norm_call(const at::Tensor& x, const c10::optional<at::Tensor>& w, const c10::optional<at::Tensor>& b, double eps,
+                   const char* who) {
+    check_float(x, "x");
+    TORCH_CHECK(x.dim() >= 1, "opentad_sparse_ops.", who, ": x needs an axis");
+    const int64_t c = x.size(-1);
+    TORCH_CHECK(c >= 1 && c <= 8192, "opentad_sparse_ops.", who, ": the width must be 1 to 8192, got ", c);
+    TORCH_CHECK(eps >= 0, "opentad_sparse_ops.", who, ": eps must not be negative");
+    NormCall n;
+    bool f32 = false, first = true;
+    for (const auto* p : {&w, &b}) {
+        if (!p->has_value() || !(*p)->defined()) continue;
+        const at::Tensor& t = **p;
+        check_float(t, "weight and bias");
+        TORCH_CHECK(t.device() == x.device(), "opentad_sparse_ops.", who, ": weight and bias must be on x's device");
+        TORCH_CHECK(t.dim() == 1 && t.size(0) == c, "opentad_sparse_ops.", who, ": weight and bias must have ", c, " elements");
+        const bool is32 = t.scalar_type() == at::kFloat;
+        TORCH_CHECK(is32 || t.scalar_type() == x.scalar_type(), "opentad_sparse_ops.", who,
+                    ": weight and bias must be float32 or have x's dtype");
+        TORCH_CHECK(first || is32 == f32, "opentad_sparse_ops.", who, ": weight and bias must have one dtype");
+        f32 = is32, first = false;
+        (p == &w ? n.w : n.b) = t.contiguous();
+    }
+    n.x = rows_of(x);
+    n.a.x = n.x.t.data_ptr();
+    n.a.w = ptr(n.w), n.a.b = ptr(n.b);
+    n.a.d0 = n.x.d[0], n.a.d1 = n.x.d[1], n.a.d2 = n.x.d[2];
+    n.a.s0 = n.x.s[0], n.a.s1 = n.x.s[1], n.a.s2 = n.x.s[2];
+    n.a.c = (int)c, n.a.params_f32 = f32, n.a.eps = (float)eps;
+    return n;
+}
+
+}  // namespace
+
+// layer_norm(x [..., c], weight, bias, eps, stats) -> (y, stats [rows, 2] float32 or empty)
+std::tuple<at::Tensor, at::Tensor> op_layer_norm(const at::Tensor& x, const c10::optional<at::Tensor>& w,
+                                                 const c10::optional<at::Tensor>& b, double eps, bool want_stats) {
+    NormCall n = norm_call(x, w, b, eps, "layer_norm");
+    c10::DeviceGuard g(x.device());
+    at::Tensor y = at::empty(x.sizes(), x.options());
+    at::Tensor stats = at::empty({want_stats ? row_count(x) : 0, 2}, x.options().dtype(at::kFloat));
+    n.a.stats = want_stats ? stats.data_ptr<float>() : nullptr;
+    check_status(svtad_norm(&n.a, y.data_ptr(), dtype_code(x), stream_of(x)), "layer_norm");
+    return {y, stats};
+}
+
+// layer_norm_bwd(dy, x, stats, weight, params_f32, need_x, need_w, need_b) -> (dx, dw, db), undefined where not needed
+std::tuple<at::Tensor, at::Tensor, at::Tensor> op_layer_norm_bwd(const at::Tensor& dy, const at::Tensor& x,
+                                                                 const at::Tensor& stats, const c10::optional<at::Tensor>& w,
+                                                                 bool params_f32, bool need_x, bool need_w, bool need_b) {
+    NormCall n = norm_call(x, w, c10::nullopt, 0.0, "layer_norm_bwd");
+    check_float(dy, "dy");
+    const int64_t rows = row_count(x), c = x.size(-1);
+    TORCH_CHECK(dy.sizes() == x.sizes() && dy.scalar_type() == x.scalar_type() && dy.device() == x.device(),
+                "opentad_sparse_ops.layer_norm_bwd: dy must be like x");
+    TORCH_CHECK(stats.is_contiguous() && stats.scalar_type() == at::kFloat && stats.numel() == 2 * rows &&
+                    stats.device() == x.device(),
+                "opentad_sparse_ops.layer_norm_bwd: stats must be the forward's");
+    TORCH_CHECK(!n.w.defined() || (n.w.scalar_type() == at::kFloat) == params_f32 || x.scalar_type() == at::kFloat,
+                "opentad_sparse_ops.layer_norm_bwd: params_f32 does not match the weight");
+    c10::DeviceGuard g(x.device());
+    // dy's rows along x's axes: the same split, or both dense
+    Rows d = rows_of(dy);
+    if (d.d[0] != n.x.d[0] || d.d[1] != n.x.d[1] || d.d[2] != n.x.d[2]) {
+        auto flat = [rows](const Rows& r) { return r.d[1] == 1 && r.d[2] == 1 && r.d[0] == rows; };
+        if (!flat(d)) d = rows_of(dy.contiguous());
+        if (!flat(n.x)) {  // dy has one stride: the same rows along x's axes
+            const int64_t s = d.s[0];
+            for (int i = 0; i < 3; ++i) d.d[i] = n.x.d[i];
+            d.s[2] = s, d.s[1] = s * d.d[2], d.s[0] = s * d.d[2] * d.d[1];
+        }
+    }
+    n.a.t0 = d.s[0], n.a.t1 = d.s[1], n.a.t2 = d.s[2];
+    n.a.stats = stats.data_ptr<float>();
+    n.a.params_f32 = params_f32;
+    at::Tensor dx, dw, db;
+    const auto param = x.options().dtype(params_f32 ? at::kFloat : x.scalar_type());
+    if (need_x) dx = at::empty(x.sizes(), x.options());
+    if (need_w) dw = at::empty({c}, param);
+    if (need_b) db = at::empty({c}, param);
+    const size_t bytes = need_w || need_b ? svtad_norm_bwd_workspace_bytes(rows, (int)c, dtype_code(x)) : 0;
+    at::Tensor ws = workspace(bytes, x);
+    check_status(svtad_norm_bwd(&n.a, d.t.data_ptr(), ptr(dx), ptr(dw), ptr(db), ptr(ws), bytes, dtype_code(x), stream_of(x)),
+                 "layer_norm_bwd");
+    return {dx, dw, db};
+}
+
+namespace {
+
+struct CrossCall {
+    svtad_cross_args a{};
+    at::Tensor q, k, v;
+};
+
+at::Tensor unit_last(const at::Tensor& t) { return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+
+CrossCall cross_call(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const c10::optional<at::Tensor>& lengths,
+                     const c10::optional<at::Tensor>& mask, double scale, const char* who) {
+    check_float(q, "q");
+    check_float(k, "k");
+    check_float(v, "v");
+    TORCH_CHECK(q.dim() == 4 && k.dim() == 4, "opentad_sparse_ops.", who, ": q and k must be [batch, tokens, heads, head_dim]");
+    TORCH_CHECK(k.sizes() == v.sizes(), "opentad_sparse_ops.", who, ": k and v must have one shape, got ", k.sizes(), " and ",
+                v.sizes());
+    TORCH_CHECK(q.size(0) == k.size(0) && q.size(3) == k.size(3), "opentad_sparse_ops.", who,
+                ": q and k must have one batch and one head dimension, got ", q.sizes(), " and ", k.sizes());
+    TORCH_CHECK(q.scalar_type() == k.scalar_type() && q.scalar_type() == v.scalar_type(), "opentad_sparse_ops.", who,
+                ": q, k and v must have one dtype");
+    TORCH_CHECK(q.device() == k.device() && q.device() == v.device(), "opentad_sparse_ops.", who,
+                ": q, k and v must be on one device");
+    TORCH_CHECK(q.size(0) <= INT32_MAX && q.size(2) <= INT32_MAX && k.size(2) <= INT32_MAX, "opentad_sparse_ops.", who,
+                ": batch or head count too large");
+    CrossCall c;
+    c.q = unit_last(q), c.k = unit_last(k), c.v = unit_last(v);
+    for (int i = 0; i < 3; ++i) {
+        c.a.q_stride[i] = c.q.stride(i);
+        c.a.k_stride[i] = c.k.stride(i);
+        c.a.v_stride[i] = c.v.stride(i);
+    }
+    c.a.q = c.q.data_ptr(), c.a.k = c.k.data_ptr(), c.a.v = c.v.data_ptr();
+    c.a.batch = q.size(0), c.a.nq = q.size(1), c.a.nk = k.size(1);
+    c.a.heads = (int)q.size(2), c.a.kv_heads = (int)k.size(2);
+    TORCH_CHECK(q.size(3) >= 1 && q.size(3) <= 128, "opentad_sparse_ops.", who, ": the head dimension must be 1 to 128, got ",
+                q.size(3));
+    c.a.head_dim = (int)q.size(3);
+    c.a.scale = (float)scale;
+    if (lengths.has_value() && lengths->defined()) {
+        TORCH_CHECK(lengths->is_cuda() && lengths->device() == q.device() && lengths->scalar_type() == at::kInt &&
+                        lengths->dim() == 1 && lengths->size(0) == q.size(0) && lengths->is_contiguous(),
+                    "opentad_sparse_ops.", who, ": key_lengths must be contiguous int32 [batch] on q's device");
+        c.a.lengths = lengths->data_ptr<int32_t>();
+    }
+    if (mask.has_value() && mask->defined()) {
+        TORCH_CHECK(mask->is_cuda() && mask->device() == q.device() && mask->scalar_type() == at::kBool && mask->dim() == 2 &&
+                        mask->size(0) == q.size(0) && mask->size(1) == k.size(1),
+                    "opentad_sparse_ops.", who, ": key_mask must be bool [batch, keys] on q's device");
+        c.a.mask = (const uint8_t*)mask->data_ptr();
+        c.a.mask_stride[0] = mask->stride(0), c.a.mask_stride[1] = mask->stride(1);
+    }
+    return c;
+}
+
+}  // namespace
+
+// cross_attention(q, k, v, key_lengths, key_mask, scale, want_lse) -> (out, lse: one float32 per row, for the backward, or empty)
+std::tuple<at::Tensor, at::Tensor> op_cross_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                      const c10::optional<at::Tensor>& lengths,
+                                                      const c10::optional<at::Tensor>& mask, double scale, bool want_lse) {
+    CrossCall c = cross_call(q, k, v, lengths, mask, scale, "cross_attention");
+    c10::DeviceGuard g(q.device());
+    const int dt = dtype_code(q);
+    at::Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+    at::Tensor lse = at::empty({want_lse ? q.size(0) : 0, q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
+    const size_t bytes = svtad_cross_attention_workspace_bytes(&c.a, dt);
+    at::Tensor ws = workspace(bytes, q);
+    check_status(svtad_cross_attention(&c.a, out.data_ptr(), want_lse ? lse.data_ptr<float>() : nullptr, ptr(ws), bytes, dt,
+                                       stream_of(q)),
+                 "cross_attention");
+    return {out, lse};
+}
+
+// cross_attention_bwd(dout, q, k, v, out, lse, key_lengths, key_mask, scale, need_q, need_kv) -> (dq, dk, dv)
+std::tuple<at::Tensor, at::Tensor, at::Tensor> op_cross_attention_bwd(
+    const at::Tensor& dout_in, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& out,
+    const at::Tensor& lse, const c10::optional<at::Tensor>& lengths, const c10::optional<at::Tensor>& mask, double scale,
+    bool need_q, bool need_kv) {
+    CrossCall c = cross_call(q, k, v, lengths, mask, scale, "cross_attention_bwd");
+    for (const at::Tensor* t : {&dout_in, &out})
+        TORCH_CHECK(t->sizes() == q.sizes() && t->scalar_type() == q.scalar_type() && t->device() == q.device(),
+                    "opentad_sparse_ops.cross_attention_bwd: dout and out must be like q");
+    TORCH_CHECK(out.is_contiguous() && lse.is_contiguous() && lse.scalar_type() == at::kFloat &&
+                    lse.numel() == q.size(0) * q.size(1) * q.size(2) && lse.device() == q.device(),
+                "opentad_sparse_ops.cross_attention_bwd: out and lse must be the forward's");
+    c10::DeviceGuard g(q.device());
+    const int dt = dtype_code(q);
+    const at::Tensor dout = unit_last(dout_in);
+    const int64_t ds[3] = {dout.stride(0), dout.stride(1), dout.stride(2)};
+    const auto dense = [](const at::Tensor& t) { return at::empty(t.sizes(), t.options()); };
+    at::Tensor dq, dk, dv;
+    if (need_q) dq = dense(q);
+    if (need_kv) dk = dense(k), dv = dense(v);
+    const size_t bytes = svtad_cross_attention_bwd_workspace_bytes(&c.a, dt);
+    at::Tensor ws = workspace(bytes, q);
+    check_status(svtad_cross_attention_bwd(&c.a, out.data_ptr(), lse.data_ptr<float>(), dout.data_ptr(), ds, ptr(dq), ptr(dk),
+                                           ptr(dv), ptr(ws), bytes, dt, stream_of(q)),
+                 "cross_attention_bwd");
+    return {dq, dk, dv};
+}
+
+// grad_clip(grads, outs (empty: the norm alone), max_norm (negative: no limit), scale, inf) -> norm, a float32 scalar
+at::Tensor op_grad_clip(const std::vector<at::Tensor>& grads, const std::vector<at::Tensor>& outs, double max_norm,
+                        double scale, bool inf) {
+    TORCH_CHECK(!grads.empty(), "opentad_sparse_ops.grad_clip: no tensors");
+    const bool write = !outs.empty();
+    TORCH_CHECK(!write || outs.size() == grads.size(), "opentad_sparse_ops.grad_clip: ", grads.size(), " gradients and ",
+                outs.size(), " outputs");
+    std::vector<svtad_grad> list(grads.size());
+    for (size_t i = 0; i < grads.size(); ++i) {
+        const at::Tensor& t = grads[i];
+        check_float(t, "gradients");
+        TORCH_CHECK(t.device() == grads[0].device(), "opentad_sparse_ops.grad_clip: gradients must be on one device");
+        TORCH_CHECK(t.is_non_overlapping_and_dense(), "opentad_sparse_ops.grad_clip: gradients must be dense");
+        list[i].g = t.data_ptr(), list[i].count = t.numel(), list[i].g_type = dtype_code(t);
+        if (!write) continue;
+        const at::Tensor& o = outs[i];
+        check_float(o, "outputs");
+        TORCH_CHECK(o.device() == t.device() && o.sizes() == t.sizes() &&
+                        ((o.is_contiguous() && t.is_contiguous()) || o.strides() == t.strides()),
+                    "opentad_sparse_ops.grad_clip: an output must have its gradient's device, shape and strides");
+        TORCH_CHECK(t.numel() == 0 || o.data_ptr() != t.data_ptr() || o.scalar_type() == t.scalar_type(),
+                    "opentad_sparse_ops.grad_clip: in place an output must have its gradient's dtype");
+        list[i].out = o.data_ptr(), list[i].out_type = dtype_code(o);
+    }
+    c10::DeviceGuard g(grads[0].device());
+    at::Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
+    const size_t bytes = svtad_grad_clip_workspace_bytes(list.data(), (int64_t)list.size());
+    at::Tensor ws = workspace(bytes, grads[0]);
+    check_status(svtad_grad_clip(list.data(), (int64_t)list.size(), inf ? SVTAD_NORM_INF : SVTAD_NORM_2, (float)max_norm,
+                                 (float)scale, write, norm.data_ptr<float>(), ptr(ws), bytes, stream_of(grads[0])),
+                 "grad_clip");
+    return norm;
+}
+
+void bind_operators(pybind11::module& m) {
+    m.def("layer_norm", &op_layer_norm, "Layer norm over the last axis (y, stats)", py::arg("x"), py::arg("weight"),
+          py::arg("bias"), py::arg("eps"), py::arg("stats"));
+    m.def("layer_norm_bwd", &op_layer_norm_bwd, "Its gradients (dx, dw, db)", py::arg("dy"), py::arg("x"), py::arg("stats"),
+          py::arg("weight"), py::arg("params_f32"), py::arg("need_x"), py::arg("need_w"), py::arg("need_b"));
+    m.def("cross_attention", &op_cross_attention, "Attention of queries to the keys of another sequence (out, lse)",
+          py::arg("q"), py::arg("k"), py::arg("v"), py::arg("key_lengths"), py::arg("key_mask"), py::arg("scale"),
+          py::arg("want_lse"));
+    m.def("cross_attention_bwd", &op_cross_attention_bwd, "Its gradients (dq, dk, dv)", py::arg("dout"), py::arg("q"),
+          py::arg("k"), py::arg("v"), py::arg("out"), py::arg("lse"), py::arg("key_lengths"), py::arg("key_mask"),
+          py::arg("scale"), py::arg("need_q"), py::arg("need_kv"));
+    m.def("grad_clip", &op_grad_clip, "The norm over all gradients, and the gradients scaled down to a limit",
+          py::arg("grads"), py::arg("outs"), py::arg("max_norm"), py::arg("scale"), py::arg("inf"));
+}

@@ -660,6 +660,91 @@ int svtad_key_attention_bwd(const void* dout, const void* q, const void* kv, con
                             size_t workspace_bytes, int64_t batch, int64_t n, int nk, int head_dim, float eps, int dtype,
                             int param_f32, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Operators of the transformer around the adapter (no counterpart in the
+ * reference's extension: its models call torch for them). dtype is
+ * SVTAD_F32, SVTAD_F16 or SVTAD_BF16; addresses need the alignment of an
+ * element only.
+ * ------------------------------------------------------------------------ */
+
+/*
+ * Layer norm over the last axis of rows x [d0, d1, d2, c] (element strides s0,
+ * s1, s2 and 1): y = (x - mean) / sqrt(var + eps) * w + b, y dense. w and b
+ * [c] may be NULL (1 and 0); they have x's type, or float32 with params_f32.
+ * c is 1 to 8192. `stats` [rows, 2] receives mean and 1 / sqrt(var + eps) of
+ * each row (NULL: not kept) and is what svtad_norm_bwd reads; dy has strides
+ * t0, t1, t2 and 1. dx (dense), dw and db may be NULL; dw and db have w's type
+ * (float32 with params_f32), are summed in float32 in a fixed order and
+ * rounded once. The workspace is needed with dw or db.
+ */
+typedef struct {
+    const void* x;
+    const void* w;
+    const void* b;
+    float* stats;
+    int64_t d0, d1, d2;
+    int64_t s0, s1, s2;
+    int64_t t0, t1, t2;
+    int c;
+    int params_f32;
+    float eps;
+} svtad_norm_args;
+int svtad_norm(const svtad_norm_args* args, void* y, int dtype, void* stream);
+size_t svtad_norm_bwd_workspace_bytes(int64_t rows, int c, int dtype);
+int svtad_norm_bwd(const svtad_norm_args* args, const void* dy, void* dx, void* dw, void* db, void* workspace,
+                   size_t workspace_bytes, int dtype, void* stream);
+
+/*
+ * Cross attention: q [batch, nq, heads, head_dim] attends to k, v [batch, nk,
+ * kv_heads, head_dim] (element strides of the first three axes given, the last
+ * 1), head h to key head h / (heads / kv_heads). Sample b sees its first
+ * lengths[b] keys (NULL: nk; clamped to 0 .. nk) where mask[b, n] is nonzero
+ * (NULL: all). out [batch, nq, heads, head_dim] is dense. A row that sees no
+ * key is 0 and has no gradient; what lies in unseen keys is never used.
+ * head_dim is 1 to 128, scale is positive. lse [batch, kv_heads, nq * heads /
+ * kv_heads] (NULL: not kept) is what the backward needs beside out. dq, dk, dv
+ * are dense; dq may be NULL, dk and dv both. Sums and softmax statistics are
+ * float32 in a fixed order; probabilities and score gradients are rounded to
+ * dtype as operands of the matrix units.
+ */
+typedef struct {
+    const void* q;
+    const void* k;
+    const void* v;
+    const int32_t* lengths;
+    const uint8_t* mask;
+    int64_t q_stride[3], k_stride[3], v_stride[3], mask_stride[2];
+    int64_t batch, nq, nk;
+    int heads, kv_heads, head_dim;
+    float scale;
+} svtad_cross_args;
+size_t svtad_cross_attention_workspace_bytes(const svtad_cross_args* args, int dtype);
+int svtad_cross_attention(const svtad_cross_args* args, void* out, float* lse, void* workspace, size_t workspace_bytes,
+                          int dtype, void* stream);
+size_t svtad_cross_attention_bwd_workspace_bytes(const svtad_cross_args* args, int dtype);
+int svtad_cross_attention_bwd(const svtad_cross_args* args, const void* out, const float* lse, const void* dout,
+                              const int64_t* dout_stride, void* dq, void* dk, void* dv, void* workspace,
+                              size_t workspace_bytes, int dtype, void* stream);
+
+/*
+ * Gradient clipping over `count` tensors (host array of descriptors; dense
+ * elements, any mix of types). norm[0] = |scale| * (2-norm of all elements, or
+ * their largest magnitude); with `write`, out = g * scale * min(1, max_norm /
+ * (norm + 1e-6)), rounded once to out_type; out may be g. A negative max_norm
+ * scales without a limit. Squares are summed in float64 in a fixed order.
+ */
+enum svtad_grad_norm { SVTAD_NORM_2 = 0, SVTAD_NORM_INF = 1 };
+typedef struct {
+    const void* g;
+    void* out;
+    int64_t count;
+    int g_type;
+    int out_type;
+} svtad_grad;
+size_t svtad_grad_clip_workspace_bytes(const svtad_grad* tensors, int64_t count);
+int svtad_grad_clip(const svtad_grad* tensors, int64_t count, int norm_type, float max_norm, float scale, int write,
+                    float* norm, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -55,8 +55,15 @@ def obj_path(src):
     return os.path.join(PKG, "_build", os.path.basename(src) + ".o")
 
 
+# accumulators of the attention kernels stay in ordinary registers: the softmax
+# rescales them between products, and from accumulation registers each such
+# use is a move there and back (a third of the loop's instructions)
+FILE_FLAGS = {"cross_attn": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+
+
 def hip_compile_cmd(src):
-    return [HIPCC, *HIP_FLAGS, "-c", src, "-o", obj_path(src)]
+    extra = [f for k, v in FILE_FLAGS.items() if os.path.basename(src).startswith(k) for f in v]
+    return [HIPCC, *HIP_FLAGS, *extra, "-c", src, "-o", obj_path(src)]
 
 
 def hip_link_cmd():

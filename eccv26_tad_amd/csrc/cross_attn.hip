@@ -51,6 +51,13 @@ static size_t bwd_bytes(const svtad_cross_args& a) {
     return align256((size_t)all_rows(a) * 4) + std::max(pq, pk);
 }
 
+// Offsets within a tile of 128 tokens, over the heads of one key head, are 32
+// bits in the kernels.
+static bool near_strides(const int64_t* s, int group, int dtype) {
+    const double size = dtype == SVTAD_F32 ? 4 : 2;
+    return s[1] >= 0 && s[2] >= 0 && ((double)s[1] * 128 + (double)s[2] * group + 128) * size < 2147483648.0;
+}
+
 static int cross_check(const svtad_cross_args* a, int dtype) {
     if (!a) return set_error(SVTAD_ERR_INVALID, "cross_attention: args is NULL");
     if (dtype != SVTAD_F32 && dtype != SVTAD_F16 && dtype != SVTAD_BF16)
@@ -66,7 +73,17 @@ static int cross_check(const svtad_cross_args* a, int dtype) {
     if ((m / 16 + 1) * bk * kMaxSplits > INT32_MAX || ((double)a->nk / 64 + 1) * bk * kMaxSplits > INT32_MAX ||
         bk * std::max(m, (double)a->nk) * 64 > (double)INT32_MAX * 256)
         return set_error(SVTAD_ERR_UNSUPPORTED, "cross_attention: too many rows or keys for one launch");
+    const int g = a->heads / a->kv_heads;
+    if (!near_strides(a->q_stride, g, dtype) || !near_strides(a->k_stride, 1, dtype) || !near_strides(a->v_stride, 1, dtype))
+        return set_error(SVTAD_ERR_UNSUPPORTED, "cross_attention: 128 tokens must lie within 2 GiB");
     return SVTAD_OK;
+}
+
+// Whether rows are read 16 bytes at a time: every start at 16 bytes and every
+// stride (of an axis with more than one place) a multiple of 8 elements.
+static bool whole_vectors(const svtad_cross_args& a, const void* p, const int64_t* s, int64_t tokens, int heads) {
+    return (uintptr_t)p % 16 == 0 && (a.batch <= 1 || s[0] % 8 == 0) && (tokens <= 1 || s[1] % 8 == 0) &&
+           (heads <= 1 || s[2] % 8 == 0);
 }
 
 static CrossArgs cross_args(const svtad_cross_args& a) {
@@ -81,6 +98,9 @@ static CrossArgs cross_args(const svtad_cross_args& a) {
     p.Nq = a.nq, p.Nk = a.nk, p.M = a.nq * p.G;
     p.scale = a.scale;
     p.c = (float)((double)a.scale * 1.4426950408889634);
+    p.inv_g = 1.f / p.G;
+    p.vec = a.head_dim % 8 == 0 && whole_vectors(a, a.q, a.q_stride, a.nq, a.heads) &&
+            whole_vectors(a, a.k, a.k_stride, a.nk, a.kv_heads) && whole_vectors(a, a.v, a.v_stride, a.nk, a.kv_heads);
     p.splits = 1;
     return p;
 }
@@ -145,6 +165,9 @@ extern "C" int svtad_cross_attention_bwd(const svtad_cross_args* a, const void* 
     CrossArgs p = cross_args(*a);
     p.o = out, p.on = (int64_t)a->heads * a->head_dim, p.oh = a->head_dim, p.ob = a->nq * p.on;
     p.dout = dout;
+    if (dout_stride && !near_strides(dout_stride, p.G, dtype))
+        return set_error(SVTAD_ERR_UNSUPPORTED, "cross_attention_bwd: 128 tokens of dout must lie within 2 GiB");
+    p.vec = p.vec && (uintptr_t)out % 16 == 0 && (!dout_stride || whole_vectors(*a, dout, dout_stride, a->nq, a->heads));
     if (dout_stride) p.gb = dout_stride[0], p.gn = dout_stride[1], p.gh = dout_stride[2];
     p.out = dq, p.dk = dk, p.dv = dv;
     p.lse = const_cast<float*>(lse);

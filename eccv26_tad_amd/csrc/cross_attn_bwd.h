@@ -17,7 +17,7 @@
 
 namespace svtad {
 
-template <typename T, int DP, int WM, int R>
+template <typename T, int DP, int WM, int R, bool VEC>
 __global__ __launch_bounds__(256) void k_cross_bwd_q(CrossArgs p) {
     constexpr int W = DP < 32 ? 32 : DP, KS = W / 32, DB = DP / 16, P = kPitch<T, W>;
     constexpr int WK = 4 / WM, TK = kTileKeys<WM>, KW = TK / WK, NB = KW / 16, ROWS = WM * R * 16;
@@ -35,9 +35,9 @@ __global__ __launch_bounds__(256) void k_cross_bwd_q(CrossArgs p) {
     t /= row_tiles;
     const int split = (int)(t % p.splits);
     const int bh = (int)(t / p.splits), b = bh / p.KH, j = bh - b * p.KH;
-    const int64_t len = seen_length(p, b);
-    const int64_t tiles = cdiv(len, TK), per = cdiv(tiles, p.splits);
-    const int64_t t0 = split * per, t1 = p.out ? min(tiles, t0 + per) : t0;
+    KeyTiles<T, TK, W, VEC> keys(p, b, j);
+    const int64_t tiles = cdiv(keys.len, TK), per = cdiv(tiles, p.splits);
+    const int64_t t0 = split * per, t1 = p.out ? lesser(tiles, t0 + per) : t0;
 
     Frag8<T> qf[R][KS], df[R][KS];
     float lse[R], delta[R];
@@ -52,10 +52,10 @@ __global__ __launch_bounds__(256) void k_cross_bwd_q(CrossArgs p) {
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             const int c = ks * 32 + g * 8;
-            qf[i][ks] = in ? load_frag<T>(q, c, p.D) : zero_frag<T>();
-            df[i][ks] = in ? load_frag<T>(d, c, p.D) : zero_frag<T>();
+            qf[i][ks] = load_frag<T, VEC>(q, c, in ? p.D : 0);
+            df[i][ks] = load_frag<T, VEC>(d, c, in ? p.D : 0);
             const Pack<T, 8> x = __builtin_bit_cast(Pack<T, 8>, df[i][ks]);
-            const Pack<T, 8> y = __builtin_bit_cast(Pack<T, 8>, in ? load_frag<T>(o, c, p.D) : zero_frag<T>());
+            const Pack<T, 8> y = __builtin_bit_cast(Pack<T, 8>, load_frag<T, VEC>(o, c, in ? p.D : 0));
 #pragma unroll
             for (int e = 0; e < 8; ++e) s = fmaf((float)x.e[e], (float)y.e[e], s);
         }
@@ -65,32 +65,26 @@ __global__ __launch_bounds__(256) void k_cross_bwd_q(CrossArgs p) {
     }
     if (!p.out) return;
 
-    const T* const kbase = (const T*)p.k + b * p.kb + j * p.kh;
-    const T* const vbase = (const T*)p.v + b * p.vb + j * p.vh;
-    const uint8_t* const mbase = p.mask ? p.mask + b * p.mask_b : nullptr;
-    auto is_seen = [&](int64_t key) { return key < len && (!mbase || mbase[key * p.mask_n]); };
-    Stage<T, TK, W> sk, sv;
-    bool ms = false;
-    auto fetch = [&](int64_t tile) {
-        sk.load([&](int r) { const int64_t key = tile * TK + r; return is_seen(key) ? kbase + key * p.kn : nullptr; }, p.D);
-        sv.load([&](int r) { const int64_t key = tile * TK + r; return is_seen(key) ? vbase + key * p.vn : nullptr; }, p.D);
-        if (mbase && threadIdx.x < TK) ms = is_seen(tile * TK + threadIdx.x);
-    };
     f32x4 acc[DB][R];
 #pragma unroll
     for (int i = 0; i < R; ++i)
 #pragma unroll
         for (int db = 0; db < DB; ++db) acc[db][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (t0 < t1) fetch(t0);
+    if (t0 < t1) {
+        keys.fetch_mask(p, t0);
+        keys.fetch(p, t0);
+        keys.fetch_mask(p, lesser(t0 + 1, t1 - 1));
+    }
     for (int64_t tile = t0; tile < t1; ++tile) {
         __syncthreads();
-        sk.store(lk);
-        sv.store(lv);
-        if (mbase && threadIdx.x < TK) seen[threadIdx.x] = ms;
+        keys.store(lk, lv, seen);
         __syncthreads();
-        if (tile + 1 < t1) fetch(tile + 1);
-        const int left = (int)min<int64_t>(len - tile * TK, TK) - wk * KW - 4 * g;
-        const bool part_seen = mbase || (tile + 1) * TK > len;
+        if (tile + 1 < t1) {
+            keys.fetch(p, tile + 1);
+            keys.fetch_mask(p, lesser(tile + 2, t1 - 1));
+        }
+        const int left = keys.left(tile) - wk * KW - 4 * g;
+        const bool part_seen = keys.mask || (tile + 1) * TK > keys.len;
 #pragma unroll
         for (int kg = 0; kg < NB / 2; ++kg) {
             f32x4 ds[2][R];
@@ -99,7 +93,10 @@ __global__ __launch_bounds__(256) void k_cross_bwd_q(CrossArgs p) {
                 const int row = wk * KW + kg * 32 + h * 16;
                 f32x4 s[R], dp[R];
 #pragma unroll
-                for (int i = 0; i < R; ++i) s[i] = dp[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int i = 0; i < R; ++i) {
+                    s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    dp[i] = f32x4{-delta[i], -delta[i], -delta[i], -delta[i]};  // the product's own sum: dp - delta
+                }
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
                     const Frag8<T> a = lds_frag<T>(lk + (row + li) * P + ks * 32 + g * 8);
@@ -110,7 +107,7 @@ __global__ __launch_bounds__(256) void k_cross_bwd_q(CrossArgs p) {
                         dp[i] = mma<T>(v, df[i][ks], dp[i]);
                     }
                 }
-                const uint32_t w = mbase ? *(const uint32_t*)(seen + row + 4 * g) : 0x01010101u;
+                const uint32_t w = keys.mask ? *(const uint32_t*)(seen + row + 4 * g) : 0x01010101u;
 #pragma unroll
                 for (int i = 0; i < R; ++i)
 #pragma unroll
@@ -118,7 +115,7 @@ __global__ __launch_bounds__(256) void k_cross_bwd_q(CrossArgs p) {
                         float pr = __builtin_amdgcn_exp2f(fmaf(s[i][e], p.c, -lse[i]));
                         // a key that is not seen was staged as zeros: its score is 0, not -inf
                         if (part_seen) pr = kg * 32 + h * 16 + e < left && ((w >> (8 * e)) & 0xff) ? pr : 0.f;
-                        ds[h][i][e] = pr * (dp[i][e] - delta[i]);
+                        ds[h][i][e] = pr * dp[i][e];
                     }
             }
             Frag8<T> sf[R];
@@ -173,7 +170,7 @@ __global__ __launch_bounds__(256) void k_cross_bwd_q(CrossArgs p) {
 // rows in tiles of kTileRows.
 constexpr int kTileRows = 64;
 
-template <typename T, int DP, int R>
+template <typename T, int DP, int R, bool VEC>
 __global__ __launch_bounds__(256) void k_cross_bwd_kv(CrossArgs p) {
     constexpr int W = DP < 32 ? 32 : DP, KS = W / 32, DB = DP / 16, P = kPitch<T, W>, TQ = kTileRows, KEYS = 64 * R;
     __shared__ __attribute__((aligned(16))) unsigned char mem[2 * (size_t)TQ * P * sizeof(T)];
@@ -190,7 +187,7 @@ __global__ __launch_bounds__(256) void k_cross_bwd_kv(CrossArgs p) {
     const int bh = (int)(t / p.splits), b = bh / p.KH, j = bh - b * p.KH;
     const int64_t len = seen_length(p, b);
     const int64_t tiles = cdiv(p.M, TQ), per = cdiv(tiles, p.splits);
-    const int64_t t0 = split * per, t1 = n0 < len ? min(tiles, t0 + per) : t0;
+    const int64_t t0 = split * per, t1 = n0 < len ? lesser(tiles, t0 + per) : t0;
 
     const uint8_t* const mbase = p.mask ? p.mask + b * p.mask_b : nullptr;
     Frag8<T> kf[R][KS], vf[R][KS];
@@ -203,22 +200,29 @@ __global__ __launch_bounds__(256) void k_cross_bwd_kv(CrossArgs p) {
         const T* const v = (const T*)p.v + b * p.vb + j * p.vh + (seen[i] ? n * p.vn : 0);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            kf[i][ks] = seen[i] ? load_frag<T>(k, ks * 32 + g * 8, p.D) : zero_frag<T>();
-            vf[i][ks] = seen[i] ? load_frag<T>(v, ks * 32 + g * 8, p.D) : zero_frag<T>();
+            kf[i][ks] = load_frag<T, VEC>(k, ks * 32 + g * 8, seen[i] ? p.D : 0);
+            vf[i][ks] = load_frag<T, VEC>(v, ks * 32 + g * 8, seen[i] ? p.D : 0);
         }
     }
 
-    const T* const qbase = (const T*)p.q + b * p.qb;
-    const T* const dbase = (const T*)p.dout + b * p.gb;
-    Stage<T, TQ, W> sq, sd;
+    const T* const qbase = (const T*)p.q + b * p.qb + (int64_t)j * p.G * p.qh;
+    const T* const dbase = (const T*)p.dout + b * p.gb + (int64_t)j * p.G * p.gh;
+    Stage<T, TQ, W, VEC> sq, sd;
     float vl = 0.f, vd = 0.f;
     auto fetch = [&](int64_t tile) {
-        sq.load([&](int i) { const int64_t r = tile * TQ + i; return r < p.M ? qbase + row_at(p, r, p.qn, p.qh, j) : nullptr; }, p.D);
-        sd.load([&](int i) { const int64_t r = tile * TQ + i; return r < p.M ? dbase + row_at(p, r, p.gn, p.gh, j) : nullptr; }, p.D);
+        const RowTile rt = row_tile(p, tile * TQ);
+        const int n = (int)lesser<int64_t>(p.M - tile * TQ, TQ);
+        const rsrc_t rq = open_rsrc(qbase + rt.n0 * p.qn), rd = open_rsrc(dbase + rt.n0 * p.gn);
+#pragma unroll
+        for (int i = 0; i < sq.kChunks; ++i) {
+            const int r = sq.row(i);
+            sq.load(i, rq, r < n ? row_tile_at(p, rt, r, p.qn, p.qh, sizeof(T)) : kOOB, p.D);
+            sd.load(i, rd, r < n ? row_tile_at(p, rt, r, p.gn, p.gh, sizeof(T)) : kOOB, p.D);
+        }
         if (threadIdx.x < TQ) {
             const int64_t r = tile * TQ + threadIdx.x;
             vl = r < p.M ? p.lse[bh * p.M + r] : -kNegInf;  // past the end: probabilities 0
-            vd = r < p.M ? p.delta[bh * p.M + r] : 0.f;
+            vd = r < p.M ? -p.delta[bh * p.M + r] : 0.f;
         }
     };
     f32x4 dk[DB][R], dv[DB][R];
@@ -244,8 +248,12 @@ __global__ __launch_bounds__(256) void k_cross_bwd_kv(CrossArgs p) {
             for (int h = 0; h < 2; ++h) {
                 const int row = rg * 32 + h * 16;
                 f32x4 s[R], dp[R];
+                const f32x4 l4 = *(const f32x4*)(ll + row + 4 * g), d4 = *(const f32x4*)(lde + row + 4 * g);
 #pragma unroll
-                for (int i = 0; i < R; ++i) s[i] = dp[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int i = 0; i < R; ++i) {
+                    s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    dp[i] = d4;  // -delta: the product's own sum is dp - delta
+                }
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
                     const Frag8<T> a = lds_frag<T>(lq + (row + li) * P + ks * 32 + g * 8);
@@ -256,7 +264,6 @@ __global__ __launch_bounds__(256) void k_cross_bwd_kv(CrossArgs p) {
                         dp[i] = mma<T>(d, vf[i][ks], dp[i]);
                     }
                 }
-                const f32x4 l4 = *(const f32x4*)(ll + row + 4 * g), d4 = *(const f32x4*)(lde + row + 4 * g);
                 // A lane's scores are all of one key: those of a key that is
                 // not seen stay in its own columns, which are stored as zeros.
 #pragma unroll
@@ -264,7 +271,7 @@ __global__ __launch_bounds__(256) void k_cross_bwd_kv(CrossArgs p) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         pr[h][i][e] = __builtin_amdgcn_exp2f(fmaf(s[i][e], p.c, -l4[e]));
-                        ds[h][i][e] = pr[h][i][e] * (dp[i][e] - d4[e]);
+                        ds[h][i][e] = pr[h][i][e] * dp[i][e];
                     }
             }
             Frag8<T> pf[R], sf[R];
@@ -347,11 +354,14 @@ __global__ __launch_bounds__(256) void k_cross_sum_kv(CrossArgs p) {
 
 template <typename T, int WM, int R>
 static void launch_cross_bwd_q(const CrossArgs& p, hipStream_t st) {
-    const int64_t grid = cdiv(p.M, WM * R * 16) * p.B * p.KH * p.splits;
-    if (p.D <= 16) k_cross_bwd_q<T, 16, WM, R><<<(unsigned)grid, 256, 0, st>>>(p);
-    else if (p.D <= 32) k_cross_bwd_q<T, 32, WM, R><<<(unsigned)grid, 256, 0, st>>>(p);
-    else if (p.D <= 64) k_cross_bwd_q<T, 64, WM, R><<<(unsigned)grid, 256, 0, st>>>(p);
-    else k_cross_bwd_q<T, 128, WM, R><<<(unsigned)grid, 256, 0, st>>>(p);
+    const unsigned grid = (unsigned)(cdiv(p.M, WM * R * 16) * p.B * p.KH * p.splits);
+    if (!p.vec) {
+        if (p.D <= 32) k_cross_bwd_q<T, 32, WM, R, false><<<grid, 256, 0, st>>>(p);
+        else k_cross_bwd_q<T, 128, WM, R, false><<<grid, 256, 0, st>>>(p);
+    } else if (p.D <= 16) k_cross_bwd_q<T, 16, WM, R, true><<<grid, 256, 0, st>>>(p);
+    else if (p.D <= 32) k_cross_bwd_q<T, 32, WM, R, true><<<grid, 256, 0, st>>>(p);
+    else if (p.D <= 64) k_cross_bwd_q<T, 64, WM, R, true><<<grid, 256, 0, st>>>(p);
+    else k_cross_bwd_q<T, 128, WM, R, true><<<grid, 256, 0, st>>>(p);
 }
 
 template <typename T>
@@ -367,11 +377,15 @@ void cross_bwd_q(const CrossArgs& p, int wave_rows, hipStream_t st) {
 
 template <typename T>
 void cross_bwd_kv(const CrossArgs& p, hipStream_t st) {
-    const int64_t grid = cdiv(p.Nk, cross_kv_keys(p.D)) * p.B * p.KH * p.splits;
-    if (p.D <= 16) k_cross_bwd_kv<T, 16, 2><<<(unsigned)grid, 256, 0, st>>>(p);
-    else if (p.D <= 32) k_cross_bwd_kv<T, 32, 2><<<(unsigned)grid, 256, 0, st>>>(p);
-    else if (p.D <= 64) k_cross_bwd_kv<T, 64, 2><<<(unsigned)grid, 256, 0, st>>>(p);
-    else k_cross_bwd_kv<T, 128, 1><<<(unsigned)grid, 256, 0, st>>>(p);
+    const unsigned grid = (unsigned)(cdiv(p.Nk, cross_kv_keys(p.D)) * p.B * p.KH * p.splits);
+    if (!p.vec) {
+        if (p.D <= 32) k_cross_bwd_kv<T, 32, 2, false><<<grid, 256, 0, st>>>(p);
+        else if (p.D <= 64) k_cross_bwd_kv<T, 64, 2, false><<<grid, 256, 0, st>>>(p);
+        else k_cross_bwd_kv<T, 128, 1, false><<<grid, 256, 0, st>>>(p);
+    } else if (p.D <= 16) k_cross_bwd_kv<T, 16, 2, true><<<grid, 256, 0, st>>>(p);
+    else if (p.D <= 32) k_cross_bwd_kv<T, 32, 2, true><<<grid, 256, 0, st>>>(p);
+    else if (p.D <= 64) k_cross_bwd_kv<T, 64, 2, true><<<grid, 256, 0, st>>>(p);
+    else k_cross_bwd_kv<T, 128, 1, true><<<grid, 256, 0, st>>>(p);
     if (p.splits > 1) {
         const int64_t n = 2 * (int64_t)p.B * p.KH * p.Nk * ((p.D + 3) / 4);
         k_cross_sum_kv<T><<<(unsigned)cdiv(n, 256), 256, 0, st>>>(p);

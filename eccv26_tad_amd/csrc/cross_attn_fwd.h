@@ -26,32 +26,52 @@ constexpr float kNegInf = -__builtin_huge_valf();
 // Keys of a staged tile: 64, or 32 per wave where the waves share a tile.
 template <int WM> constexpr int kTileKeys = WM == 1 ? 128 : 64;
 
-// One thread's share of a tile of TILE rows by W elements: loads to registers
-// and stores to LDS. Rows for which `row` gives NULL are zeros.
-template <typename T, int TILE, int W>
-struct Stage {
-    static constexpr int kChunks = TILE * W / 8 / 256;
-    Frag8<T> v[kChunks];
+// The keys of one sample and key head as a workgroup walks over them: tiles of
+// keys and values on their way to LDS, and which keys are seen.
+template <typename T, int TK, int W, bool VEC>
+struct KeyTiles {
+    Stage<T, TK, W, VEC> sk, sv;
+    const T *k, *v;
+    const uint8_t* mask;
+    int64_t len;
+    uint8_t next[Stage<T, TK, W, VEC>::kChunks];  // the mask at the next tile's rows
+    uint8_t own, own_next;                        // and at row threadIdx.x
 
-    template <typename F>
-    __device__ __forceinline__ void load(F row, int d) {
+    __device__ __forceinline__ KeyTiles(const CrossArgs& p, int b, int j)
+        : k((const T*)p.k + b * p.kb + j * p.kh), v((const T*)p.v + b * p.vb + j * p.vh),
+          mask(p.mask ? p.mask + b * p.mask_b : nullptr), len(seen_length(p, b)) {}
+
+    __device__ __forceinline__ int left(int64_t tile) const { return (int)lesser<int64_t>(len - tile * TK, TK); }
+
+    // The mask is read a tile ahead of the rows whose loads depend on it.
+    __device__ __forceinline__ void fetch_mask(const CrossArgs& p, int64_t tile) {
+        if (!mask) return;
+        const int n = left(tile);
+        const uint8_t* const m = mask + tile * TK * p.mask_n;
 #pragma unroll
-        for (int i = 0; i < kChunks; ++i) {
-            const int ch = threadIdx.x + i * 256, r = ch / (W / 8), c = ch % (W / 8) * 8;
-            const T* const at = row(r);
-            v[i] = at ? load_frag<T>(at, c, d) : zero_frag<T>();
-        }
+        for (int i = 0; i < sk.kChunks; ++i) next[i] = sk.row(i) < n ? m[sk.row(i) * p.mask_n] : 0;
+        own_next = (int)threadIdx.x < lesser(n, TK) ? m[threadIdx.x * p.mask_n] : 0;
     }
-    __device__ __forceinline__ void store(T* lds) const {
+    __device__ __forceinline__ void fetch(const CrossArgs& p, int64_t tile) {
+        const int n = left(tile);
+        const rsrc_t rk = open_rsrc(k + tile * TK * p.kn), rv = open_rsrc(v + tile * TK * p.vn);
 #pragma unroll
-        for (int i = 0; i < kChunks; ++i) {
-            const int ch = threadIdx.x + i * 256, r = ch / (W / 8), c = ch % (W / 8) * 8;
-            *(Frag8<T>*)(lds + r * kPitch<T, W> + c) = v[i];
+        for (int i = 0; i < sk.kChunks; ++i) {
+            const int r = sk.row(i);
+            const bool in = r < n && (!mask || next[i]);
+            sk.load(i, rk, in ? (uint32_t)(r * (int)p.kn) * (int)sizeof(T) : kOOB, p.D);
+            sv.load(i, rv, in ? (uint32_t)(r * (int)p.vn) * (int)sizeof(T) : kOOB, p.D);
         }
+        own = own_next;
+    }
+    __device__ __forceinline__ void store(T* lk, T* lv, uint8_t* seen) {
+        sk.store(lk);
+        sv.store(lv);
+        if (mask && threadIdx.x < TK) seen[threadIdx.x] = own;
     }
 };
 
-template <typename T, int DP, int WM, int R>
+template <typename T, int DP, int WM, int R, bool VEC>
 __global__ __launch_bounds__(256) void k_cross_fwd(CrossArgs p) {
     constexpr int W = DP < 32 ? 32 : DP, KS = W / 32, DB = DP / 16, P = kPitch<T, W>;
     constexpr int WK = 4 / WM, TK = kTileKeys<WM>, KW = TK / WK, NB = KW / 16, ROWS = WM * R * 16;
@@ -70,9 +90,9 @@ __global__ __launch_bounds__(256) void k_cross_fwd(CrossArgs p) {
     t /= row_tiles;
     const int split = (int)(t % p.splits);
     const int bh = (int)(t / p.splits), b = bh / p.KH, j = bh - b * p.KH;
-    const int64_t len = seen_length(p, b);
-    const int64_t tiles = cdiv(len, TK), per = cdiv(tiles, p.splits);
-    const int64_t t0 = split * per, t1 = min(tiles, t0 + per);
+    KeyTiles<T, TK, W, VEC> keys(p, b, j);
+    const int64_t tiles = cdiv(keys.len, TK), per = cdiv(tiles, p.splits);
+    const int64_t t0 = split * per, t1 = lesser(tiles, t0 + per);
 
     Frag8<T> qf[R][KS];
 #pragma unroll
@@ -80,20 +100,8 @@ __global__ __launch_bounds__(256) void k_cross_fwd(CrossArgs p) {
         const int64_t r = r0 + (wm * R + i) * 16 + li;
         const T* const q = (const T*)p.q + b * p.qb + (r < p.M ? row_at(p, r, p.qn, p.qh, j) : 0);
 #pragma unroll
-        for (int s = 0; s < KS; ++s) qf[i][s] = r < p.M ? load_frag<T>(q, s * 32 + g * 8, p.D) : zero_frag<T>();
+        for (int s = 0; s < KS; ++s) qf[i][s] = load_frag<T, VEC>(q, s * 32 + g * 8, r < p.M ? p.D : 0);
     }
-
-    const T* const kbase = (const T*)p.k + b * p.kb + j * p.kh;
-    const T* const vbase = (const T*)p.v + b * p.vb + j * p.vh;
-    const uint8_t* const mbase = p.mask ? p.mask + b * p.mask_b : nullptr;
-    auto is_seen = [&](int64_t key) { return key < len && (!mbase || mbase[key * p.mask_n]); };
-    Stage<T, TK, W> sk, sv;
-    bool ms = false;
-    auto fetch = [&](int64_t tile) {
-        sk.load([&](int r) { const int64_t key = tile * TK + r; return is_seen(key) ? kbase + key * p.kn : nullptr; }, p.D);
-        sv.load([&](int r) { const int64_t key = tile * TK + r; return is_seen(key) ? vbase + key * p.vn : nullptr; }, p.D);
-        if (mbase && threadIdx.x < TK) ms = is_seen(tile * TK + threadIdx.x);
-    };
 
     f32x4 acc[DB][R];
     float m[R], l[R];
@@ -103,14 +111,19 @@ __global__ __launch_bounds__(256) void k_cross_fwd(CrossArgs p) {
 #pragma unroll
         for (int db = 0; db < DB; ++db) acc[db][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    if (t0 < t1) fetch(t0);
+    if (t0 < t1) {
+        keys.fetch_mask(p, t0);
+        keys.fetch(p, t0);
+        keys.fetch_mask(p, lesser(t0 + 1, t1 - 1));
+    }
     for (int64_t tile = t0; tile < t1; ++tile) {
         __syncthreads();
-        sk.store(lk);
-        sv.store(lv);
-        if (mbase && threadIdx.x < TK) seen[threadIdx.x] = ms;
+        keys.store(lk, lv, seen);
         __syncthreads();
-        if (tile + 1 < t1) fetch(tile + 1);
+        if (tile + 1 < t1) {
+            keys.fetch(p, tile + 1);
+            keys.fetch_mask(p, lesser(tile + 2, t1 - 1));
+        }
 
         f32x4 s[NB][R];
 #pragma unroll
@@ -124,7 +137,7 @@ __global__ __launch_bounds__(256) void k_cross_fwd(CrossArgs p) {
                 for (int i = 0; i < R; ++i) s[nb][i] = mma<T>(a, qf[i][ks], s[nb][i]);
             }
         }
-        if (mbase) {
+        if (keys.mask) {
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
                 const uint32_t w = *(const uint32_t*)(seen + wk * KW + nb * 16 + 4 * g);
@@ -133,8 +146,8 @@ __global__ __launch_bounds__(256) void k_cross_fwd(CrossArgs p) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) s[nb][i][e] = (w >> (8 * e)) & 0xff ? s[nb][i][e] : kNegInf;
             }
-        } else if ((tile + 1) * TK > len) {
-            const int left = (int)(len - tile * TK) - wk * KW - 4 * g;
+        } else if ((tile + 1) * TK > keys.len) {
+            const int left = keys.left(tile) - wk * KW - 4 * g;
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -275,11 +288,14 @@ __global__ __launch_bounds__(256) void k_cross_join(CrossArgs p) {
 
 template <typename T, int WM, int R>
 static void launch_cross_fwd(const CrossArgs& p, hipStream_t st) {
-    const int64_t grid = cdiv(p.M, WM * R * 16) * p.B * p.KH * p.splits;
-    if (p.D <= 16) k_cross_fwd<T, 16, WM, R><<<(unsigned)grid, 256, 0, st>>>(p);
-    else if (p.D <= 32) k_cross_fwd<T, 32, WM, R><<<(unsigned)grid, 256, 0, st>>>(p);
-    else if (p.D <= 64) k_cross_fwd<T, 64, WM, R><<<(unsigned)grid, 256, 0, st>>>(p);
-    else k_cross_fwd<T, 128, WM, R><<<(unsigned)grid, 256, 0, st>>>(p);
+    const unsigned grid = (unsigned)(cdiv(p.M, WM * R * 16) * p.B * p.KH * p.splits);
+    if (!p.vec) {
+        if (p.D <= 32) k_cross_fwd<T, 32, WM, R, false><<<grid, 256, 0, st>>>(p);
+        else k_cross_fwd<T, 128, WM, R, false><<<grid, 256, 0, st>>>(p);
+    } else if (p.D <= 16) k_cross_fwd<T, 16, WM, R, true><<<grid, 256, 0, st>>>(p);
+    else if (p.D <= 32) k_cross_fwd<T, 32, WM, R, true><<<grid, 256, 0, st>>>(p);
+    else if (p.D <= 64) k_cross_fwd<T, 64, WM, R, true><<<grid, 256, 0, st>>>(p);
+    else k_cross_fwd<T, 128, WM, R, true><<<grid, 256, 0, st>>>(p);
 }
 
 template <typename T>

@@ -78,14 +78,14 @@ __global__ __launch_bounds__(256) void k_grad_norm(ClipList t, double* part) {
     const int64_t total = t.end[t.count - 1];
     const int64_t per = cdiv(cdiv(total, gridDim.x), 64) * 64;
     int64_t e = (int64_t)blockIdx.x * per;
-    const int64_t e1 = min(total, e + per);
+    const int64_t e1 = min<int64_t>(total, e + per);
     double acc = 0.0;
     auto add = [&](T v) {
         const double d = (double)(float)v;
         acc = INF ? clip_join<true>(acc, fabs(d)) : fma(d, d, acc);
     };
     for (int i = e < e1 ? clip_find(t, e) : 0; e < e1; ++i) {
-        const int64_t first = i ? t.end[i - 1] : 0, stop = min(e1, t.end[i]);
+        const int64_t first = i ? t.end[i - 1] : 0, stop = min<int64_t>(e1, t.end[i]);
         const T* const g = (const T*)t.g[i] + (e - first);
         const int64_t n = stop - e, body = n / (256 * V) * (256 * V);
         int64_t at = threadIdx.x * V;
@@ -141,9 +141,9 @@ __global__ __launch_bounds__(256) void k_grad_scale(ClipList t, ClipScale s) {
     const int64_t total = t.end[t.count - 1];
     const int64_t per = cdiv(cdiv(total, gridDim.x), 64) * 64;
     int64_t e = (int64_t)(gridDim.x - 1 - blockIdx.x) * per;
-    const int64_t e1 = min(total, e + per);
+    const int64_t e1 = min<int64_t>(total, e + per);
     for (int i = e < e1 ? clip_find(t, e) : 0; e < e1; ++i) {
-        const int64_t first = i ? t.end[i - 1] : 0, stop = min(e1, t.end[i]);
+        const int64_t first = i ? t.end[i - 1] : 0, stop = min<int64_t>(e1, t.end[i]);
         const T* const g = (const T*)t.g[i] + (e - first);
         O* const o = (O*)t.out[i] + (e - first);
         const int64_t m = stop - e, body = m / (256 * V) * (256 * V);

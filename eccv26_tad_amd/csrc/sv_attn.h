@@ -18,6 +18,11 @@
 
 namespace svtad {
 
+template <typename I>
+__device__ __forceinline__ I lesser(I a, I b) {  // in integers (an overloaded min may go by way of double)
+    return a < b ? a : b;
+}
+
 // 8 reduction values of a 16 x 16 x 32 product per lane; float32 runs it as
 // eight 16 x 16 x 4 products, whose operands pair values of equal position, so
 // the same layout serves.
@@ -46,26 +51,27 @@ template <typename T> __device__ __forceinline__ Frag8<T> zero_frag() {
     return __builtin_bit_cast(Frag8<T>, Pack<T, 8>{});
 }
 
-// 8 elements of a row of d in global memory from column c on, 0 past its end
-template <typename T>
+// 8 elements of a row of d in global memory from column c on, 0 past its end.
+// VEC: d is a multiple of 8 and rows start at 16 bytes.
+template <typename T, bool VEC>
 __device__ __forceinline__ Frag8<T> load_frag(const T* row, int c, int d) {
-    if (c + 8 <= d) return __builtin_bit_cast(Frag8<T>, *(const Pack<T, 8>*)(row + c));
-    Pack<T, 8> v;
+    if constexpr (VEC) {
+        return c < d ? *(const Frag8<T>*)(row + c) : zero_frag<T>();
+    } else {
+        Pack<T, 8> v;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v.e[e] = c + e < d ? row[c + e] : (T)0.f;
-    return __builtin_bit_cast(Frag8<T>, v);
+        for (int e = 0; e < 8; ++e) v.e[e] = c + e < d ? row[c + e] : (T)0.f;
+        return __builtin_bit_cast(Frag8<T>, v);
+    }
 }
 
 // The right operand of a 32-value product from two score tiles of a lane
+typedef float f32x8 __attribute__((ext_vector_type(8)));
 template <typename T>
 __device__ __forceinline__ Frag8<T> pack_frag(const f32x4& a, const f32x4& b) {
-    Pack<T, 8> v;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        v.e[e] = (T)a[e];
-        v.e[4 + e] = (T)b[e];
-    }
-    return __builtin_bit_cast(Frag8<T>, v);
+    typedef T tx8 __attribute__((ext_vector_type(8)));
+    const f32x8 v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_bit_cast(Frag8<T>, __builtin_convertvector(v, tx8));
 }
 
 // LDS tile of rows of DP elements; the pad spreads the 16 rows that a fragment
@@ -139,6 +145,59 @@ __device__ __forceinline__ void store4(T* row, int c, int d, f32x4 v) {
     }
 }
 
+// One thread's share of a tile of TILE rows by W elements, loaded to registers
+// through a buffer descriptor (rows that do not exist, and columns past d, read
+// as zeros without a branch) and stored to LDS.
+template <typename T, int TILE, int W, bool VEC>
+struct Stage {
+    static constexpr int kChunks = TILE * W / 8 / 256;
+    static_assert(TILE * W / 8 % 256 == 0, "whole chunks per thread");
+    Frag8<T> v[kChunks];
+
+    static __device__ __forceinline__ int row(int i) { return (threadIdx.x + i * 256) / (W / 8); }
+    static __device__ __forceinline__ int col(int i) { return (threadIdx.x + i * 256) % (W / 8) * 8; }
+
+    // chunk i of the row that starts `at` bytes into the tile (kOOB: none)
+    __device__ __forceinline__ void load(int i, rsrc_t r, uint32_t at, int d) {
+        constexpr int S = (int)sizeof(T);
+        const int c = col(i);
+        if constexpr (VEC) {
+            const uint32_t off = c < d ? at + c * S : kOOB;
+            if constexpr (S == 2) {
+                v[i].v = bload16(r, off);
+            } else {
+                union {
+                    u32x4 q[2];
+                    Frag8<T> f;
+                } u;
+                u.q[0] = bload16(r, off);
+                u.q[1] = bload16(r, off + 16);
+                v[i] = u.f;
+            }
+        } else {
+            Pack<T, 8> p;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t off = c + e < d ? at + (c + e) * S : kOOB;
+                if constexpr (S == 2) p.e[e] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0));
+                else p.e[e] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0));
+            }
+            v[i] = __builtin_bit_cast(Frag8<T>, p);
+        }
+    }
+    __device__ __forceinline__ void store(T* lds) const {
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) *(Frag8<T>*)(lds + row(i) * kPitch<T, W> + col(i)) = v[i];
+    }
+};
+
+// A descriptor from `base` on. Loads check their rows themselves and give kOOB
+// where there is none; valid offsets are below 2^31.
+template <typename T>
+__device__ __forceinline__ rsrc_t open_rsrc(const T* base) {
+    return make_rsrc(base, 0x7fffffffu);
+}
+
 // ---------------------------------------------------------------------------
 
 struct CrossArgs {
@@ -154,14 +213,33 @@ struct CrossArgs {
     int B, H, KH, G, D;    // G = H / KH query heads per key head
     int64_t Nq, Nk, M;     // M = Nq G rows per key head: row r is query r / G, head (key head) G + r % G
     int splits;            // of the reduced axis
-    float c, scale;        // scale log2(e)
+    float c, scale;        // c = scale log2(e)
+    float inv_g;           // 1 / G
+    bool vec;              // D and all strides are multiples of 8 elements, all starts of 16 bytes
 };
 
-// Row r of the M rows of key head `j`: its query and head
+// Row r of the M rows of key head `j`: the offset of its query and head
 __device__ __forceinline__ int64_t row_at(const CrossArgs& p, int64_t r, int64_t sn, int64_t sh, int j) {
     if (p.G == 1) return r * sn + j * sh;
     const uint64_t n = (uint64_t)r / (uint32_t)p.G;
     return n * sn + (int64_t)(j * p.G + (int)(r - n * p.G)) * sh;
+}
+
+// The tile of rows r0 .. r0 + 63 as offsets from its first query's address: row
+// i's bytes from there (without key head j's own offset)
+struct RowTile {
+    int64_t n0;  // first query
+    int rem;     // r0 - n0 G
+};
+__device__ __forceinline__ RowTile row_tile(const CrossArgs& p, int64_t r0) {
+    if (p.G == 1) return {r0, 0};
+    const uint64_t n = (uint64_t)r0 / (uint32_t)p.G;
+    return {(int64_t)n, (int)(r0 - n * p.G)};
+}
+__device__ __forceinline__ uint32_t row_tile_at(const CrossArgs& p, const RowTile& t, int i, int64_t sn, int64_t sh, int size) {
+    if (p.G == 1) return (uint32_t)(i * (int)sn) * size;
+    const int x = i + t.rem, n = (int)((x + 0.5f) * p.inv_g);  // x below 2^20: exact
+    return (uint32_t)(n * (int)sn + (x - n * p.G) * (int)sh) * size;
 }
 
 __device__ __forceinline__ int64_t seen_length(const CrossArgs& p, int b) {

@@ -157,7 +157,12 @@ struct CrossCall {
     at::Tensor q, k, v;
 };
 
-at::Tensor unit_last(const at::Tensor& t) { return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+// t [batch, tokens, heads, head_dim] as the kernels read it: a strided last axis,
+// or 128 tokens that lie further apart than 2 GiB, are copied
+at::Tensor readable(const at::Tensor& t, int64_t group) {
+    const double apart = ((double)t.stride(1) * 128 + (double)t.stride(2) * group + 128) * t.element_size();
+    return (t.size(-1) <= 1 || t.stride(-1) == 1) && apart < 2147483648.0 ? t : t.contiguous();
+}
 
 CrossCall cross_call(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const c10::optional<at::Tensor>& lengths,
                      const c10::optional<at::Tensor>& mask, double scale, const char* who) {
@@ -176,7 +181,8 @@ CrossCall cross_call(const at::Tensor& q, const at::Tensor& k, const at::Tensor&
     TORCH_CHECK(q.size(0) <= INT32_MAX && q.size(2) <= INT32_MAX && k.size(2) <= INT32_MAX, "opentad_sparse_ops.", who,
                 ": batch or head count too large");
     CrossCall c;
-    c.q = unit_last(q), c.k = unit_last(k), c.v = unit_last(v);
+    const int64_t group = k.size(2) > 0 ? q.size(2) / k.size(2) : 1;
+    c.q = readable(q, group), c.k = readable(k, 1), c.v = readable(v, 1);
     for (int i = 0; i < 3; ++i) {
         c.a.q_stride[i] = c.q.stride(i);
         c.a.k_stride[i] = c.k.stride(i);
@@ -238,7 +244,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> op_cross_attention_bwd(
                 "opentad_sparse_ops.cross_attention_bwd: out and lse must be the forward's");
     c10::DeviceGuard g(q.device());
     const int dt = dtype_code(q);
-    const at::Tensor dout = unit_last(dout_in);
+    const at::Tensor dout = readable(dout_in, q.size(2) / k.size(2));
     const int64_t ds[3] = {dout.stride(0), dout.stride(1), dout.stride(2)};
     const auto dense = [](const at::Tensor& t) { return at::empty(t.sizes(), t.options()); };
     at::Tensor dq, dk, dv;

@@ -19,26 +19,20 @@ namespace svtad {
 
 template <typename T, int DP, int WM, int R, bool VEC>
 __global__ __launch_bounds__(256) void k_cross_bwd_q(CrossArgs p) {
-    constexpr int W = DP < 32 ? 32 : DP, KS = W / 32, DB = DP / 16, P = kPitch<T, W>;
+    constexpr int W = DP < 32 ? 32 : DP, KS = W / 32, DB = DP / 16;
     constexpr int WK = 4 / WM, TK = kTileKeys<WM>, KW = TK / WK, NB = KW / 16, ROWS = WM * R * 16;
-    constexpr size_t kTiles = 2 * (size_t)TK * P * sizeof(T), kJoin = WK > 1 ? (size_t)WK * ROWS * DP * 4 : 0;
-    __shared__ __attribute__((aligned(16))) unsigned char mem[kTiles > kJoin ? kTiles : kJoin];
-    __shared__ __attribute__((aligned(16))) uint8_t seen[TK];
-    T* const lk = (T*)mem;
-    T* const lv = lk + TK * P;
+    typedef LdsTile<T, W> Tile;
+    typedef KeyTiles<T, TK, W, VEC> Keys;
+    constexpr size_t kJoin = WK > 1 ? (size_t)WK * ROWS * DP * 4 : 0;
+    __shared__ __attribute__((aligned(16))) unsigned char mem[Keys::kBytes > kJoin ? Keys::kBytes : kJoin];
+    __shared__ __attribute__((aligned(16))) uint8_t seen_mem[Keys::kBuffers * TK];
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave % WM, wk = wave / WM;
     const int g = lane >> 4, li = lane & 15;
     const int64_t row_tiles = cdiv(p.M, ROWS);
-    int64_t t = xcd_tile(blockIdx.x, gridDim.x);
-    const int64_t r0 = t % row_tiles * ROWS;
-    t /= row_tiles;
-    const int split = (int)(t % p.splits);
-    const int bh = (int)(t / p.splits), b = bh / p.KH, j = bh - b * p.KH;
-    KeyTiles<T, TK, W, VEC> keys(p, b, j);
-    const int64_t tiles = cdiv(keys.len, TK), per = cdiv(tiles, p.splits);
-    const int64_t t0 = split * per, t1 = p.out ? lesser(tiles, t0 + per) : t0;
-
+    const HeadTile ht = head_tile(blockIdx.x, gridDim.x, row_tiles * p.splits);
+    const int bh = ht.bh, b = bh / p.KH, j = bh - b * p.KH, split = (int)(ht.tile / row_tiles);
+    const int64_t r0 = (ht.tile - split * row_tiles) * ROWS;
     Frag8<T> qf[R][KS], df[R][KS];
     float lse[R], delta[R];
 #pragma unroll
@@ -70,19 +64,9 @@ __global__ __launch_bounds__(256) void k_cross_bwd_q(CrossArgs p) {
     for (int i = 0; i < R; ++i)
 #pragma unroll
         for (int db = 0; db < DB; ++db) acc[db][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (t0 < t1) {
-        keys.fetch_mask(p, t0);
-        keys.fetch(p, t0);
-        keys.fetch_mask(p, lesser(t0 + 1, t1 - 1));
-    }
-    for (int64_t tile = t0; tile < t1; ++tile) {
-        __syncthreads();
-        keys.store(lk, lv, seen);
-        __syncthreads();
-        if (tile + 1 < t1) {
-            keys.fetch(p, tile + 1);
-            keys.fetch_mask(p, lesser(tile + 2, t1 - 1));
-        }
+    Keys keys(p, b, j, split, mem, seen_mem);
+    keys.walk(p, [&](int64_t tile) {
+        const unsigned char *const lk = keys.keys(tile), *const lv = keys.values(tile);
         const int left = keys.left(tile) - wk * KW - 4 * g;
         const bool part_seen = keys.mask || (tile + 1) * TK > keys.len;
 #pragma unroll
@@ -99,36 +83,39 @@ __global__ __launch_bounds__(256) void k_cross_bwd_q(CrossArgs p) {
                 }
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
-                    const Frag8<T> a = lds_frag<T>(lk + (row + li) * P + ks * 32 + g * 8);
-                    const Frag8<T> v = lds_frag<T>(lv + (row + li) * P + ks * 32 + g * 8);
+                    const Frag8<T> a = Tile::frag(lk, row, ks, lane);
+                    const Frag8<T> v = Tile::frag(lv, row, ks, lane);
 #pragma unroll
                     for (int i = 0; i < R; ++i) {
                         s[i] = mma<T>(a, qf[i][ks], s[i]);
                         dp[i] = mma<T>(v, df[i][ks], dp[i]);
                     }
                 }
-                const uint32_t w = keys.mask ? *(const uint32_t*)(seen + row + 4 * g) : 0x01010101u;
+                if (part_seen) {  // an unseen key was staged as zeros: its score is 0, not -inf
+                    const uint32_t w = keys.mask ? *(const uint32_t*)(keys.seen(tile) + row + 4 * g) : 0x01010101u;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const bool in = kg * 32 + h * 16 + e < left && ((w >> (8 * e)) & 0xff);
+#pragma unroll
+                        for (int i = 0; i < R; ++i) s[i][e] = in ? s[i][e] : kNegInf;
+                    }
+                }
 #pragma unroll
                 for (int i = 0; i < R; ++i)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float pr = __builtin_amdgcn_exp2f(fmaf(s[i][e], p.c, -lse[i]));
-                        // a key that is not seen was staged as zeros: its score is 0, not -inf
-                        if (part_seen) pr = kg * 32 + h * 16 + e < left && ((w >> (8 * e)) & 0xff) ? pr : 0.f;
-                        ds[h][i][e] = pr * dp[i][e];
-                    }
+                    for (int e = 0; e < 4; ++e) ds[h][i][e] = __builtin_amdgcn_exp2f(fmaf(s[i][e], p.c, -lse[i])) * dp[i][e];
             }
             Frag8<T> sf[R];
 #pragma unroll
             for (int i = 0; i < R; ++i) sf[i] = pack_frag<T>(ds[0][i], ds[1][i]);
 #pragma unroll
             for (int db = 0; db < DB; ++db) {
-                const Frag8<T> a = lds_frag_t<T, P>(lk + (wk * KW + kg * 32) * P, db * 16, lane);
+                const Frag8<T> a = Tile::frag_t(lk, wk * KW + kg * 32, db, lane);
 #pragma unroll
                 for (int i = 0; i < R; ++i) acc[db][i] = mma<T>(a, sf[i], acc[db][i]);
             }
         }
-    }
+    });
 
     if constexpr (WK > 1) {  // add the waves of equal rows, in order
         float* const jo = (float*)mem;  // [WK][ROWS][DP]
@@ -172,19 +159,18 @@ constexpr int kTileRows = 64;
 
 template <typename T, int DP, int R, bool VEC>
 __global__ __launch_bounds__(256) void k_cross_bwd_kv(CrossArgs p) {
-    constexpr int W = DP < 32 ? 32 : DP, KS = W / 32, DB = DP / 16, P = kPitch<T, W>, TQ = kTileRows, KEYS = 64 * R;
-    __shared__ __attribute__((aligned(16))) unsigned char mem[2 * (size_t)TQ * P * sizeof(T)];
-    __shared__ __attribute__((aligned(16))) float ll[TQ], lde[TQ];
-    T* const lq = (T*)mem;
-    T* const ld = lq + TQ * P;
+    constexpr int W = DP < 32 ? 32 : DP, KS = W / 32, DB = DP / 16, TQ = kTileRows, KEYS = 64 * R;
+    typedef LdsTile<T, W> Tile;
+    typedef Stage<T, TQ, W, VEC> S;
+    // two tiles of rows: one is read while the next arrives
+    __shared__ __attribute__((aligned(16))) unsigned char mem[2][2][S::kBytes];  // [buffer][q, dout]
+    __shared__ __attribute__((aligned(16))) float ll[2][TQ], lde[2][TQ];
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, li = lane & 15;
     const int64_t key_tiles = cdiv(p.Nk, KEYS);
-    int64_t t = xcd_tile(blockIdx.x, gridDim.x);
-    const int64_t n0 = t % key_tiles * KEYS;
-    t /= key_tiles;
-    const int split = (int)(t % p.splits);
-    const int bh = (int)(t / p.splits), b = bh / p.KH, j = bh - b * p.KH;
+    const HeadTile ht = head_tile(blockIdx.x, gridDim.x, key_tiles * p.splits);
+    const int bh = ht.bh, b = bh / p.KH, j = bh - b * p.KH, split = (int)(ht.tile / key_tiles);
+    const int64_t n0 = (ht.tile - split * key_tiles) * KEYS;
     const int64_t len = seen_length(p, b);
     const int64_t tiles = cdiv(p.M, TQ), per = cdiv(tiles, p.splits);
     const int64_t t0 = split * per, t1 = n0 < len ? lesser(tiles, t0 + per) : t0;
@@ -207,40 +193,42 @@ __global__ __launch_bounds__(256) void k_cross_bwd_kv(CrossArgs p) {
 
     const T* const qbase = (const T*)p.q + b * p.qb + (int64_t)j * p.G * p.qh;
     const T* const dbase = (const T*)p.dout + b * p.gb + (int64_t)j * p.G * p.gh;
-    Stage<T, TQ, W, VEC> sq, sd;
-    float vl = 0.f, vd = 0.f;
+    S sq, sd;
     auto fetch = [&](int64_t tile) {
         const RowTile rt = row_tile(p, tile * TQ);
         const int n = (int)lesser<int64_t>(p.M - tile * TQ, TQ);
         const rsrc_t rq = open_rsrc(qbase + rt.n0 * p.qn), rd = open_rsrc(dbase + rt.n0 * p.gn);
 #pragma unroll
-        for (int i = 0; i < sq.kChunks; ++i) {
-            const int r = sq.row(i);
-            sq.load(i, rq, r < n ? row_tile_at(p, rt, r, p.qn, p.qh, sizeof(T)) : kOOB, p.D);
-            sd.load(i, rd, r < n ? row_tile_at(p, rt, r, p.gn, p.gh, sizeof(T)) : kOOB, p.D);
+        for (int i = 0; i < S::kCount; ++i) {
+            const int r = S::row(i);
+            sq.load(i, rq, r < n ? row_tile_at(p, rt, r, p.qn, p.qh, sizeof(T)) : kOOB, p.D, mem[tile & 1][0]);
+            sd.load(i, rd, r < n ? row_tile_at(p, rt, r, p.gn, p.gh, sizeof(T)) : kOOB, p.D, mem[tile & 1][1]);
         }
         if (threadIdx.x < TQ) {
             const int64_t r = tile * TQ + threadIdx.x;
-            vl = r < p.M ? p.lse[bh * p.M + r] : -kNegInf;  // past the end: probabilities 0
-            vd = r < p.M ? -p.delta[bh * p.M + r] : 0.f;
+            ll[tile & 1][threadIdx.x] = r < p.M ? p.lse[bh * p.M + r] : -kNegInf;  // past the end: probabilities 0
+            lde[tile & 1][threadIdx.x] = r < p.M ? -p.delta[bh * p.M + r] : 0.f;
         }
+    };
+    auto arrive = [&](int64_t tile) {
+        sq.store(mem[tile & 1][0]);
+        sd.store(mem[tile & 1][1]);
+        landed();
     };
     f32x4 dk[DB][R], dv[DB][R];
 #pragma unroll
     for (int i = 0; i < R; ++i)
 #pragma unroll
         for (int db = 0; db < DB; ++db) dk[db][i] = dv[db][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (t0 < t1) fetch(t0);
+    if (t0 < t1) {
+        fetch(t0);
+        arrive(t0);
+    }
     for (int64_t tile = t0; tile < t1; ++tile) {
         __syncthreads();
-        sq.store(lq);
-        sd.store(ld);
-        if (threadIdx.x < TQ) {
-            ll[threadIdx.x] = vl;
-            lde[threadIdx.x] = vd;
-        }
-        __syncthreads();
         if (tile + 1 < t1) fetch(tile + 1);
+        const unsigned char *const lq = mem[tile & 1][0], *const ld = mem[tile & 1][1];
+        const float *const l_tile = ll[tile & 1], *const d_tile = lde[tile & 1];
 #pragma unroll
         for (int rg = 0; rg < TQ / 32; ++rg) {
             f32x4 pr[2][R], ds[2][R];
@@ -248,7 +236,7 @@ __global__ __launch_bounds__(256) void k_cross_bwd_kv(CrossArgs p) {
             for (int h = 0; h < 2; ++h) {
                 const int row = rg * 32 + h * 16;
                 f32x4 s[R], dp[R];
-                const f32x4 l4 = *(const f32x4*)(ll + row + 4 * g), d4 = *(const f32x4*)(lde + row + 4 * g);
+                const f32x4 l4 = *(const f32x4*)(l_tile + row + 4 * g), d4 = *(const f32x4*)(d_tile + row + 4 * g);
 #pragma unroll
                 for (int i = 0; i < R; ++i) {
                     s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -256,8 +244,8 @@ __global__ __launch_bounds__(256) void k_cross_bwd_kv(CrossArgs p) {
                 }
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
-                    const Frag8<T> a = lds_frag<T>(lq + (row + li) * P + ks * 32 + g * 8);
-                    const Frag8<T> d = lds_frag<T>(ld + (row + li) * P + ks * 32 + g * 8);
+                    const Frag8<T> a = Tile::frag(lq, row, ks, lane);
+                    const Frag8<T> d = Tile::frag(ld, row, ks, lane);
 #pragma unroll
                     for (int i = 0; i < R; ++i) {
                         s[i] = mma<T>(a, kf[i][ks], s[i]);
@@ -282,8 +270,8 @@ __global__ __launch_bounds__(256) void k_cross_bwd_kv(CrossArgs p) {
             }
 #pragma unroll
             for (int db = 0; db < DB; ++db) {
-                const Frag8<T> d = lds_frag_t<T, P>(ld + rg * 32 * P, db * 16, lane);
-                const Frag8<T> a = lds_frag_t<T, P>(lq + rg * 32 * P, db * 16, lane);
+                const Frag8<T> d = Tile::frag_t(ld, rg * 32, db, lane);
+                const Frag8<T> a = Tile::frag_t(lq, rg * 32, db, lane);
 #pragma unroll
                 for (int i = 0; i < R; ++i) {
                     dv[db][i] = mma<T>(d, pf[i], dv[db][i]);
@@ -291,6 +279,7 @@ __global__ __launch_bounds__(256) void k_cross_bwd_kv(CrossArgs p) {
                 }
             }
         }
+        if (tile + 1 < t1) arrive(tile + 1);
     }
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll

@@ -27,72 +27,106 @@ constexpr float kNegInf = -__builtin_huge_valf();
 template <int WM> constexpr int kTileKeys = WM == 1 ? 128 : 64;
 
 // The keys of one sample and key head as a workgroup walks over them: tiles of
-// keys and values on their way to LDS, and which keys are seen.
+// TK keys and values in LDS, two of them where they fit (one is read while the
+// next arrives), and which keys are seen.
 template <typename T, int TK, int W, bool VEC>
 struct KeyTiles {
-    Stage<T, TK, W, VEC> sk, sv;
+    typedef Stage<T, TK, W, VEC> S;
+    static constexpr int kTile = 2 * S::kBytes, kBuffers = 2 * kTile <= 128 * 1024 ? 2 : 1;
+    static constexpr size_t kBytes = (size_t)kBuffers * kTile;
+    S sk, sv;
     const T *k, *v;
     const uint8_t* mask;
-    int64_t len;
-    uint8_t next[Stage<T, TK, W, VEC>::kChunks];  // the mask at the next tile's rows
-    uint8_t own, own_next;                        // and at row threadIdx.x
+    int64_t len, t0, t1;
+    unsigned char* mem;     // [kBuffers][K, V]
+    uint8_t* seen_mem;      // [kBuffers][TK]
+    uint8_t next[S::kCount];  // the mask at the next tile's rows
+    uint8_t own;              // and at row threadIdx.x
 
-    __device__ __forceinline__ KeyTiles(const CrossArgs& p, int b, int j)
+    __device__ __forceinline__ KeyTiles(const CrossArgs& p, int b, int j, int split, unsigned char* mem, uint8_t* seen_mem)
         : k((const T*)p.k + b * p.kb + j * p.kh), v((const T*)p.v + b * p.vb + j * p.vh),
-          mask(p.mask ? p.mask + b * p.mask_b : nullptr), len(seen_length(p, b)) {}
+          mask(p.mask ? p.mask + b * p.mask_b : nullptr), len(seen_length(p, b)), mem(mem), seen_mem(seen_mem) {
+        const int64_t tiles = cdiv(len, TK), per = cdiv(tiles, p.splits);
+        t0 = split * per, t1 = lesser(tiles, t0 + per);
+    }
 
     __device__ __forceinline__ int left(int64_t tile) const { return (int)lesser<int64_t>(len - tile * TK, TK); }
+    __device__ __forceinline__ unsigned char* keys(int64_t tile) const { return mem + (kBuffers == 2 ? (int)(tile & 1) * kTile : 0); }
+    __device__ __forceinline__ unsigned char* values(int64_t tile) const { return keys(tile) + S::kBytes; }
+    __device__ __forceinline__ uint8_t* seen(int64_t tile) const { return seen_mem + (kBuffers == 2 ? (int)(tile & 1) * TK : 0); }
 
     // The mask is read a tile ahead of the rows whose loads depend on it.
     __device__ __forceinline__ void fetch_mask(const CrossArgs& p, int64_t tile) {
-        if (!mask) return;
+        if (!mask || tile >= t1) return;
         const int n = left(tile);
         const uint8_t* const m = mask + tile * TK * p.mask_n;
 #pragma unroll
-        for (int i = 0; i < sk.kChunks; ++i) next[i] = sk.row(i) < n ? m[sk.row(i) * p.mask_n] : 0;
-        own_next = (int)threadIdx.x < lesser(n, TK) ? m[threadIdx.x * p.mask_n] : 0;
+        for (int i = 0; i < S::kCount; ++i) next[i] = S::row(i) < n ? m[S::row(i) * p.mask_n] : 0;
+        own = (int)threadIdx.x < n ? m[threadIdx.x * p.mask_n] : 0;  // n is at most TK
     }
     __device__ __forceinline__ void fetch(const CrossArgs& p, int64_t tile) {
         const int n = left(tile);
         const rsrc_t rk = open_rsrc(k + tile * TK * p.kn), rv = open_rsrc(v + tile * TK * p.vn);
 #pragma unroll
-        for (int i = 0; i < sk.kChunks; ++i) {
-            const int r = sk.row(i);
+        for (int i = 0; i < S::kCount; ++i) {
+            const int r = S::row(i);
             const bool in = r < n && (!mask || next[i]);
-            sk.load(i, rk, in ? (uint32_t)(r * (int)p.kn) * (int)sizeof(T) : kOOB, p.D);
-            sv.load(i, rv, in ? (uint32_t)(r * (int)p.vn) * (int)sizeof(T) : kOOB, p.D);
+            sk.load(i, rk, in ? (uint32_t)(r * (int)p.kn) * (int)sizeof(T) : kOOB, p.D, keys(tile));
+            sv.load(i, rv, in ? (uint32_t)(r * (int)p.vn) * (int)sizeof(T) : kOOB, p.D, values(tile));
         }
-        own = own_next;
+        if (mask && threadIdx.x < TK) seen(tile)[threadIdx.x] = own;
+        fetch_mask(p, tile + 1);
     }
-    __device__ __forceinline__ void store(T* lk, T* lv, uint8_t* seen) {
-        sk.store(lk);
-        sv.store(lv);
-        if (mask && threadIdx.x < TK) seen[threadIdx.x] = own;
+    __device__ __forceinline__ void arrive(int64_t tile) {
+        sk.store(keys(tile));
+        sv.store(values(tile));
+        landed();
+    }
+
+    // All tiles of this split, `use` on each
+    template <typename F>
+    __device__ __forceinline__ void walk(const CrossArgs& p, F use) {
+        if (t0 >= t1) return;
+        fetch_mask(p, t0);
+        if constexpr (kBuffers == 2) {
+            fetch(p, t0);
+            arrive(t0);
+            for (int64_t tile = t0; tile < t1; ++tile) {
+                __syncthreads();  // this tile has arrived, and nobody reads the other any more
+                if (tile + 1 < t1) fetch(p, tile + 1);
+                use(tile);
+                if (tile + 1 < t1) arrive(tile + 1);
+            }
+        } else {
+            for (int64_t tile = t0; tile < t1; ++tile) {
+                __syncthreads();
+                fetch(p, tile);
+                arrive(tile);
+                __syncthreads();
+                use(tile);
+            }
+        }
     }
 };
 
 template <typename T, int DP, int WM, int R, bool VEC>
 __global__ __launch_bounds__(256) void k_cross_fwd(CrossArgs p) {
-    constexpr int W = DP < 32 ? 32 : DP, KS = W / 32, DB = DP / 16, P = kPitch<T, W>;
+    constexpr int W = DP < 32 ? 32 : DP, KS = W / 32, DB = DP / 16;
     constexpr int WK = 4 / WM, TK = kTileKeys<WM>, KW = TK / WK, NB = KW / 16, ROWS = WM * R * 16;
     static_assert(KW % 32 == 0, "a wave's keys fill whole products");
-    constexpr size_t kTiles = 2 * (size_t)TK * P * sizeof(T), kJoin = WK > 1 ? (size_t)WK * ROWS * (DP + 2) * 4 : 0;
-    __shared__ __attribute__((aligned(16))) unsigned char mem[kTiles > kJoin ? kTiles : kJoin];
-    __shared__ __attribute__((aligned(16))) uint8_t seen[TK];
-    T* const lk = (T*)mem;
-    T* const lv = lk + TK * P;
+    typedef LdsTile<T, W> Tile;
+    typedef KeyTiles<T, TK, W, VEC> Keys;
+    constexpr size_t kJoin = WK > 1 ? (size_t)WK * ROWS * (DP + 2) * 4 : 0;
+    __shared__ __attribute__((aligned(16))) unsigned char mem[Keys::kBytes > kJoin ? Keys::kBytes : kJoin];
+    __shared__ __attribute__((aligned(16))) uint8_t seen_mem[Keys::kBuffers * TK];
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave % WM, wk = wave / WM;
     const int g = lane >> 4, li = lane & 15;
     const int64_t row_tiles = cdiv(p.M, ROWS);
-    int64_t t = xcd_tile(blockIdx.x, gridDim.x);
-    const int64_t r0 = t % row_tiles * ROWS;
-    t /= row_tiles;
-    const int split = (int)(t % p.splits);
-    const int bh = (int)(t / p.splits), b = bh / p.KH, j = bh - b * p.KH;
-    KeyTiles<T, TK, W, VEC> keys(p, b, j);
-    const int64_t tiles = cdiv(keys.len, TK), per = cdiv(tiles, p.splits);
-    const int64_t t0 = split * per, t1 = lesser(tiles, t0 + per);
+    const HeadTile ht = head_tile(blockIdx.x, gridDim.x, row_tiles * p.splits);
+    const int bh = ht.bh, b = bh / p.KH, j = bh - b * p.KH, split = (int)(ht.tile / row_tiles);
+    const int64_t r0 = (ht.tile - split * row_tiles) * ROWS;
+    Keys keys(p, b, j, split, mem, seen_mem);
 
     Frag8<T> qf[R][KS];
 #pragma unroll
@@ -111,20 +145,8 @@ __global__ __launch_bounds__(256) void k_cross_fwd(CrossArgs p) {
 #pragma unroll
         for (int db = 0; db < DB; ++db) acc[db][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    if (t0 < t1) {
-        keys.fetch_mask(p, t0);
-        keys.fetch(p, t0);
-        keys.fetch_mask(p, lesser(t0 + 1, t1 - 1));
-    }
-    for (int64_t tile = t0; tile < t1; ++tile) {
-        __syncthreads();
-        keys.store(lk, lv, seen);
-        __syncthreads();
-        if (tile + 1 < t1) {
-            keys.fetch(p, tile + 1);
-            keys.fetch_mask(p, lesser(tile + 2, t1 - 1));
-        }
-
+    keys.walk(p, [&](int64_t tile) {
+        const unsigned char *const lk = keys.keys(tile), *const lv = keys.values(tile);
         f32x4 s[NB][R];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
@@ -132,7 +154,7 @@ __global__ __launch_bounds__(256) void k_cross_fwd(CrossArgs p) {
             for (int i = 0; i < R; ++i) s[nb][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                const Frag8<T> a = lds_frag<T>(lk + (wk * KW + nb * 16 + li) * P + ks * 32 + g * 8);
+                const Frag8<T> a = Tile::frag(lk, wk * KW + nb * 16, ks, lane);
 #pragma unroll
                 for (int i = 0; i < R; ++i) s[nb][i] = mma<T>(a, qf[i][ks], s[nb][i]);
             }
@@ -140,7 +162,7 @@ __global__ __launch_bounds__(256) void k_cross_fwd(CrossArgs p) {
         if (keys.mask) {
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-                const uint32_t w = *(const uint32_t*)(seen + wk * KW + nb * 16 + 4 * g);
+                const uint32_t w = *(const uint32_t*)(keys.seen(tile) + wk * KW + nb * 16 + 4 * g);
 #pragma unroll
                 for (int i = 0; i < R; ++i)
 #pragma unroll
@@ -186,12 +208,12 @@ __global__ __launch_bounds__(256) void k_cross_fwd(CrossArgs p) {
             for (int i = 0; i < R; ++i) pf[i] = pack_frag<T>(s[2 * kg][i], s[2 * kg + 1][i]);
 #pragma unroll
             for (int db = 0; db < DB; ++db) {
-                const Frag8<T> a = lds_frag_t<T, P>(lv + (wk * KW + kg * 32) * P, db * 16, lane);
+                const Frag8<T> a = Tile::frag_t(lv, wk * KW + kg * 32, db, lane);
 #pragma unroll
                 for (int i = 0; i < R; ++i) acc[db][i] = mma<T>(a, pf[i], acc[db][i]);
             }
         }
-    }
+    });
 #pragma unroll
     for (int i = 0; i < R; ++i) l[i] = across_groups_sum(l[i]);
 

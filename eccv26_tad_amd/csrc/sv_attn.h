@@ -74,52 +74,71 @@ __device__ __forceinline__ Frag8<T> pack_frag(const f32x4& a, const f32x4& b) {
     return __builtin_bit_cast(Frag8<T>, __builtin_convertvector(v, tx8));
 }
 
-// LDS tile of rows of DP elements; the pad spreads the 16 rows that a fragment
-// read touches over all banks.
-template <typename T, int DP> constexpr int kPitch = DP + 16 / (int)sizeof(T);
+// A tile of rows of W elements in LDS, in pieces of 16 bytes without padding
+// (so that a wave's loads may land there directly, 64 consecutive pieces at a
+// time). Row r keeps its piece c at place c ^ swizzle(r), which spreads both
+// kinds of reads over all banks: the same piece of 16 rows (frag), and two
+// neighbouring pieces of 8 rows (frag_t), whose swizzles differ above bit 0.
+template <typename T, int W>
+struct LdsTile {
+    static constexpr int kRow = W * (int)sizeof(T), kPieces = kRow / 16, kElems = 16 / (int)sizeof(T);
+    static constexpr int kBits = kRow >= 256 ? 4 : kRow == 128 ? 3 : 2, kShift = 4 - kBits;
 
-template <typename T>
-__device__ __forceinline__ Frag8<T> lds_frag(const T* p) {  // 8 consecutive elements
-    Frag8<T> f;
-    if constexpr (sizeof(T) == 2) {
-        f.v = *(const u32x4*)p;
-    } else {
-        const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f.e[e] = a[e], f.e[4 + e] = b[e];
+    static __device__ __forceinline__ int swizzle(int r) {
+        const int e = (r & 15) >> kShift;
+        return ((e << 1) | (e >> (kBits - 1))) & ((1 << kBits) - 1);
     }
-    return f;
-}
-
-// Transposed: column `col0 + lane % 16` of rows 4g .. 4g+3 and 16 + 4g ..
-// 16 + 4g+3 below `tile` (g = lane / 16): the left operand that pairs with
-// pack_frag. For 16-bit types the transposing read: the 16 lanes of a group
-// give the addresses of 4 rows' 4 chunks and receive a column each.
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-template <typename T, int PITCH_>
-__device__ __forceinline__ Frag8<T> lds_frag_t(const T* tile, int col0, int lane) {
-    const int g = lane >> 4, i = lane & 15;
-    Frag8<T> f;
-    if constexpr (sizeof(T) == 2) {
-        typedef __attribute__((address_space(3))) s16x4* lds4;
-        const T* p = tile + (4 * g + (i >> 2)) * PITCH_ + col0 + 4 * (i & 3);
-        union {
-            s16x4 h[2];
-            u32x4 v;
-        } u;
-        u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)p);
-        u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 16 * PITCH_));
-        f.v = u.v;
-    } else {
-        const T* p = tile + 4 * g * PITCH_ + col0 + i;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            f.e[e] = p[e * PITCH_];
-            f.e[4 + e] = p[(16 + e) * PITCH_];
+    // 8 elements ks * 32 + 8 (lane / 16) .. of row r0 + lane % 16; r0 a multiple of 16
+    static __device__ __forceinline__ Frag8<T> frag(const unsigned char* tile, int r0, int ks, int lane) {
+        const int g = lane >> 4, li = lane & 15;
+        const unsigned char* const row = tile + (r0 + li) * kRow;
+        if constexpr (sizeof(T) == 2) {
+            Frag8<T> f;
+            f.v = *(const u32x4*)(row + (((ks * 4) ^ (g ^ swizzle(li))) << 4));
+            return f;
+        } else {
+            union {
+                u32x4 q[2];
+                Frag8<T> f;
+            } u;
+            const int at = (ks * 8) ^ ((2 * g) ^ swizzle(li));
+            u.q[0] = *(const u32x4*)(row + (at << 4));
+            u.q[1] = *(const u32x4*)(row + ((at ^ 1) << 4));
+            return u.f;
         }
     }
-    return f;
-}
+    // Transposed: column db * 16 + lane % 16 of rows r0 + 4g .. + 3 and r0 + 16
+    // + 4g .. + 3 (g = lane / 16): the left operand that pairs with pack_frag.
+    // For 16-bit types the transposing read: the 16 lanes of a group give the
+    // addresses of 4 rows' 4 chunks of 8 bytes and receive a column each.
+    static __device__ __forceinline__ Frag8<T> frag_t(const unsigned char* tile, int r0, int db, int lane) {
+        const int g = lane >> 4, i = lane & 15;
+        Frag8<T> f;
+        if constexpr (sizeof(T) == 2) {
+            typedef short s16x4 __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) s16x4* lds4;
+            const int r = 4 * g + (i >> 2);
+            const unsigned char* const p =
+                tile + (r0 + r) * kRow + (((db * 2) ^ (((i >> 1) & 1) ^ swizzle(r))) << 4) + 8 * (i & 1);
+            union {
+                s16x4 h[2];
+                u32x4 v;
+            } u;
+            u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)p);
+            u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 16 * kRow));
+            f.v = u.v;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = 4 * g + e;
+                const unsigned char* const p = tile + (r0 + r) * kRow + (((db * 4) ^ ((i >> 2) ^ swizzle(r))) << 4) + 4 * (i & 3);
+                f.e[e] = *(const T*)p;
+                f.e[4 + e] = *(const T*)(p + 16 * kRow);
+            }
+        }
+        return f;
+    }
+};
 
 __device__ __forceinline__ float across_groups_max(float v) {  // over lanes of equal lane % 16
     v = fmaxf(v, __shfl_xor(v, 16, 64));
@@ -145,51 +164,52 @@ __device__ __forceinline__ void store4(T* row, int c, int d, f32x4 v) {
     }
 }
 
-// One thread's share of a tile of TILE rows by W elements, loaded to registers
-// through a buffer descriptor (rows that do not exist, and columns past d, read
-// as zeros without a branch) and stored to LDS.
+// One thread's share of loading a tile of TILE rows by W elements to LDS through
+// a buffer descriptor: rows that do not exist, and columns past d, arrive as
+// zeros without a branch. VEC: straight to LDS, without registers; a barrier
+// after `landed` makes the tile readable. Otherwise element by element through
+// registers, which `store` empties into the tile.
 template <typename T, int TILE, int W, bool VEC>
 struct Stage {
-    static constexpr int kChunks = TILE * W / 8 / 256;
-    static_assert(TILE * W / 8 % 256 == 0, "whole chunks per thread");
-    Frag8<T> v[kChunks];
+    typedef LdsTile<T, W> Tile;
+    static constexpr int kCount = TILE * Tile::kPieces / 256, kBytes = TILE * Tile::kRow, E = Tile::kElems;
+    static_assert(TILE * Tile::kPieces % 256 == 0, "whole pieces per thread");
+    u32x4 v[VEC ? 1 : kCount];
 
-    static __device__ __forceinline__ int row(int i) { return (threadIdx.x + i * 256) / (W / 8); }
-    static __device__ __forceinline__ int col(int i) { return (threadIdx.x + i * 256) % (W / 8) * 8; }
+    static __device__ __forceinline__ int row(int i) { return (threadIdx.x + i * 256) / Tile::kPieces; }
+    static __device__ __forceinline__ int col(int i) {
+        return (((threadIdx.x + i * 256) % Tile::kPieces) ^ Tile::swizzle(row(i))) * E;
+    }
 
-    // chunk i of the row that starts `at` bytes into the tile (kOOB: none)
-    __device__ __forceinline__ void load(int i, rsrc_t r, uint32_t at, int d) {
+    // piece i, of a row that starts `at` bytes from the descriptor's (kOOB: none)
+    __device__ __forceinline__ void load(int i, rsrc_t r, uint32_t at, int d, unsigned char* tile) {
         constexpr int S = (int)sizeof(T);
         const int c = col(i);
         if constexpr (VEC) {
-            const uint32_t off = c < d ? at + c * S : kOOB;
-            if constexpr (S == 2) {
-                v[i].v = bload16(r, off);
-            } else {
-                union {
-                    u32x4 q[2];
-                    Frag8<T> f;
-                } u;
-                u.q[0] = bload16(r, off);
-                u.q[1] = bload16(r, off + 16);
-                v[i] = u.f;
-            }
+            typedef __attribute__((address_space(3))) void* lds;
+            unsigned char* const to = tile + (i * 256 + (threadIdx.x & ~63)) * 16;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds)to, 16, c < d ? at + c * S : kOOB, 0, 0, 0);
         } else {
-            Pack<T, 8> p;
+            Pack<T, E> p;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
+            for (int e = 0; e < E; ++e) {
                 const uint32_t off = c + e < d ? at + (c + e) * S : kOOB;
                 if constexpr (S == 2) p.e[e] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0));
                 else p.e[e] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0));
             }
-            v[i] = __builtin_bit_cast(Frag8<T>, p);
+            v[i] = __builtin_bit_cast(u32x4, p);
         }
     }
-    __device__ __forceinline__ void store(T* lds) const {
+    __device__ __forceinline__ void store(unsigned char* tile) const {
+        if constexpr (!VEC) {
 #pragma unroll
-        for (int i = 0; i < kChunks; ++i) *(Frag8<T>*)(lds + row(i) * kPitch<T, W> + col(i)) = v[i];
+            for (int i = 0; i < kCount; ++i) *(u32x4*)(tile + (threadIdx.x + i * 256) * 16) = v[i];
+        }
     }
 };
+
+// Waits for this wave's loads to LDS (which the compiler does not wait for)
+__device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // A descriptor from `base` on. Loads check their rows themselves and give kOOB
 // where there is none; valid offsets are below 2^31.
@@ -217,6 +237,24 @@ struct CrossArgs {
     float inv_g;           // 1 / G
     bool vec;              // D and all strides are multiples of 8 elements, all starts of 16 bytes
 };
+
+// Workgroup -> (sample and key head, tile): the n tiles of a head stay on one
+// XCD, whose L2 then holds its keys (workgroup w runs on XCD w % 8), and
+// neighbouring heads go to different XCDs, so that samples of unequal length
+// load all XCDs alike. The heads beyond a multiple of 8 are cut across XCDs.
+struct HeadTile {
+    int bh;
+    int64_t tile;
+};
+__device__ __forceinline__ HeadTile head_tile(int64_t w, int64_t grid, int64_t n) {
+    const int64_t eights = grid / n / 8, whole = eights * 8 * n;
+    if (w < whole) {
+        const int64_t k = w >> 3, q = k / n;
+        return {(int)(q * 8 + (w & 7)), k - q * n};
+    }
+    const int64_t t = xcd_tile(w - whole, grid - whole), q = t / n;
+    return {(int)(eights * 8 + q), t - q * n};
+}
 
 // Row r of the M rows of key head `j`: the offset of its query and head
 __device__ __forceinline__ int64_t row_at(const CrossArgs& p, int64_t r, int64_t sn, int64_t sh, int j) {

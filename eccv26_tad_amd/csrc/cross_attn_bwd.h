@@ -29,10 +29,10 @@ __global__ __launch_bounds__(256) void k_cross_bwd_q(CrossArgs p) {
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave % WM, wk = wave / WM;
     const int g = lane >> 4, li = lane & 15;
-    const int64_t row_tiles = cdiv(p.M, ROWS);
+    const uint32_t row_tiles = ((uint32_t)p.M + ROWS - 1) / ROWS;
     const HeadTile ht = head_tile(blockIdx.x, gridDim.x, row_tiles * p.splits);
     const int bh = ht.bh, b = bh / p.KH, j = bh - b * p.KH, split = (int)(ht.tile / row_tiles);
-    const int64_t r0 = (ht.tile - split * row_tiles) * ROWS;
+    const int64_t r0 = (int64_t)(ht.tile - split * row_tiles) * ROWS;
     Frag8<T> qf[R][KS], df[R][KS];
     float lse[R], delta[R];
 #pragma unroll
@@ -65,10 +65,9 @@ __global__ __launch_bounds__(256) void k_cross_bwd_q(CrossArgs p) {
 #pragma unroll
         for (int db = 0; db < DB; ++db) acc[db][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     Keys keys(p, b, j, split, mem, seen_mem);
-    keys.walk(p, [&](int64_t tile) {
+    auto use = [&](int64_t tile, auto part) __attribute__((always_inline)) {
         const unsigned char *const lk = keys.keys(tile), *const lv = keys.values(tile);
         const int left = keys.left(tile) - wk * KW - 4 * g;
-        const bool part_seen = keys.mask || (tile + 1) * TK > keys.len;
 #pragma unroll
         for (int kg = 0; kg < NB / 2; ++kg) {
             f32x4 ds[2][R];
@@ -91,7 +90,7 @@ __global__ __launch_bounds__(256) void k_cross_bwd_q(CrossArgs p) {
                         dp[i] = mma<T>(v, df[i][ks], dp[i]);
                     }
                 }
-                if (part_seen) {  // an unseen key was staged as zeros: its score is 0, not -inf
+                if constexpr (part.value) {  // an unseen key was staged as zeros: its score is 0, not -inf
                     const uint32_t w = keys.mask ? *(const uint32_t*)(keys.seen(tile) + row + 4 * g) : 0x01010101u;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -115,7 +114,8 @@ __global__ __launch_bounds__(256) void k_cross_bwd_q(CrossArgs p) {
                 for (int i = 0; i < R; ++i) acc[db][i] = mma<T>(a, sf[i], acc[db][i]);
             }
         }
-    });
+    };
+    keys.walk(p, [&](int64_t t) { use(t, std::false_type()); }, [&](int64_t t) { use(t, std::true_type()); });
 
     if constexpr (WK > 1) {  // add the waves of equal rows, in order
         float* const jo = (float*)mem;  // [WK][ROWS][DP]
@@ -167,13 +167,13 @@ __global__ __launch_bounds__(256) void k_cross_bwd_kv(CrossArgs p) {
     __shared__ __attribute__((aligned(16))) float ll[2][TQ], lde[2][TQ];
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, li = lane & 15;
-    const int64_t key_tiles = cdiv(p.Nk, KEYS);
+    const uint32_t key_tiles = (uint32_t)cdiv(p.Nk, KEYS);
     const HeadTile ht = head_tile(blockIdx.x, gridDim.x, key_tiles * p.splits);
     const int bh = ht.bh, b = bh / p.KH, j = bh - b * p.KH, split = (int)(ht.tile / key_tiles);
-    const int64_t n0 = (ht.tile - split * key_tiles) * KEYS;
+    const int64_t n0 = (int64_t)(ht.tile - split * key_tiles) * KEYS;
     const int64_t len = seen_length(p, b);
-    const int64_t tiles = cdiv(p.M, TQ), per = cdiv(tiles, p.splits);
-    const int64_t t0 = split * per, t1 = n0 < len ? lesser(tiles, t0 + per) : t0;
+    const uint32_t tiles = ((uint32_t)p.M + TQ - 1) / TQ, per = (tiles + p.splits - 1) / p.splits;
+    const int64_t t0 = split * per, t1 = n0 < len ? lesser(tiles, split * per + per) : t0;
 
     const uint8_t* const mbase = p.mask ? p.mask + b * p.mask_b : nullptr;
     Frag8<T> kf[R][KS], vf[R][KS];
@@ -197,7 +197,7 @@ __global__ __launch_bounds__(256) void k_cross_bwd_kv(CrossArgs p) {
     auto fetch = [&](int64_t tile) {
         const RowTile rt = row_tile(p, tile * TQ);
         const int n = (int)lesser<int64_t>(p.M - tile * TQ, TQ);
-        const rsrc_t rq = open_rsrc(qbase + rt.n0 * p.qn), rd = open_rsrc(dbase + rt.n0 * p.gn);
+        const Buffer rq = open_buffer(qbase + rt.n0 * p.qn), rd = open_buffer(dbase + rt.n0 * p.gn);
 #pragma unroll
         for (int i = 0; i < S::kCount; ++i) {
             const int r = S::row(i);

@@ -17,11 +17,18 @@
 // neither infinities nor NaN in their places reach a result.
 #pragma once
 
+#include <type_traits>
+
 #include "cross_attn.h"
 
 namespace svtad {
 
 constexpr float kNegInf = -__builtin_huge_valf();
+
+// The sums keep the scale of an earlier maximum until a score is 2^kSlack above
+// it: after the first tiles of a row they are hardly rescaled again (32 products
+// per tile and lane otherwise), and the powers stay below 2^kSlack.
+constexpr float kSlack = 8.f;
 
 // Keys of a staged tile: 64, or 32 per wave where the waves share a tile.
 template <int WM> constexpr int kTileKeys = WM == 1 ? 128 : 64;
@@ -46,8 +53,8 @@ struct KeyTiles {
     __device__ __forceinline__ KeyTiles(const CrossArgs& p, int b, int j, int split, unsigned char* mem, uint8_t* seen_mem)
         : k((const T*)p.k + b * p.kb + j * p.kh), v((const T*)p.v + b * p.vb + j * p.vh),
           mask(p.mask ? p.mask + b * p.mask_b : nullptr), len(seen_length(p, b)), mem(mem), seen_mem(seen_mem) {
-        const int64_t tiles = cdiv(len, TK), per = cdiv(tiles, p.splits);
-        t0 = split * per, t1 = lesser(tiles, t0 + per);
+        const uint32_t tiles = (uint32_t)cdiv(len, TK), per = (tiles + p.splits - 1) / p.splits;
+        t0 = split * per, t1 = lesser(tiles, split * per + per);
     }
 
     __device__ __forceinline__ int left(int64_t tile) const { return (int)lesser<int64_t>(len - tile * TK, TK); }
@@ -66,7 +73,7 @@ struct KeyTiles {
     }
     __device__ __forceinline__ void fetch(const CrossArgs& p, int64_t tile) {
         const int n = left(tile);
-        const rsrc_t rk = open_rsrc(k + tile * TK * p.kn), rv = open_rsrc(v + tile * TK * p.vn);
+        const Buffer rk = open_buffer(k + tile * TK * p.kn), rv = open_buffer(v + tile * TK * p.vn);
 #pragma unroll
         for (int i = 0; i < S::kCount; ++i) {
             const int r = S::row(i);
@@ -83,28 +90,33 @@ struct KeyTiles {
         landed();
     }
 
-    // All tiles of this split, `use` on each
-    template <typename F>
-    __device__ __forceinline__ void walk(const CrossArgs& p, F use) {
+    // All tiles of this split: whole(tile) on those whose keys are all seen,
+    // part(tile) on the others (the last one, or with a mask any), in loops of
+    // their own, so that neither carries the other's cases.
+    template <typename F, typename G>
+    __device__ __forceinline__ void walk(const CrossArgs& p, F whole, G part) {
         if (t0 >= t1) return;
+        const int64_t tw = mask ? t0 : max<int64_t>(t0, lesser(t1, len / TK));
         fetch_mask(p, t0);
         if constexpr (kBuffers == 2) {
             fetch(p, t0);
             arrive(t0);
-            for (int64_t tile = t0; tile < t1; ++tile) {
-                __syncthreads();  // this tile has arrived, and nobody reads the other any more
-                if (tile + 1 < t1) fetch(p, tile + 1);
-                use(tile);
-                if (tile + 1 < t1) arrive(tile + 1);
-            }
+        }
+        for (int64_t tile = t0; tile < tw; ++tile) step(p, tile, whole);
+        for (int64_t tile = tw; tile < t1; ++tile) step(p, tile, part);
+    }
+    template <typename F>
+    __device__ __forceinline__ void step(const CrossArgs& p, int64_t tile, F use) {
+        __syncthreads();  // this tile has arrived, and nobody reads the other any more
+        if constexpr (kBuffers == 2) {
+            if (tile + 1 < t1) fetch(p, tile + 1);
+            use(tile);
+            if (tile + 1 < t1) arrive(tile + 1);
         } else {
-            for (int64_t tile = t0; tile < t1; ++tile) {
-                __syncthreads();
-                fetch(p, tile);
-                arrive(tile);
-                __syncthreads();
-                use(tile);
-            }
+            fetch(p, tile);
+            arrive(tile);
+            __syncthreads();
+            use(tile);
         }
     }
 };
@@ -122,10 +134,10 @@ __global__ __launch_bounds__(256) void k_cross_fwd(CrossArgs p) {
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave % WM, wk = wave / WM;
     const int g = lane >> 4, li = lane & 15;
-    const int64_t row_tiles = cdiv(p.M, ROWS);
+    const uint32_t row_tiles = ((uint32_t)p.M + ROWS - 1) / ROWS;
     const HeadTile ht = head_tile(blockIdx.x, gridDim.x, row_tiles * p.splits);
     const int bh = ht.bh, b = bh / p.KH, j = bh - b * p.KH, split = (int)(ht.tile / row_tiles);
-    const int64_t r0 = (ht.tile - split * row_tiles) * ROWS;
+    const int64_t r0 = (int64_t)(ht.tile - split * row_tiles) * ROWS;
     Keys keys(p, b, j, split, mem, seen_mem);
 
     Frag8<T> qf[R][KS];
@@ -145,7 +157,7 @@ __global__ __launch_bounds__(256) void k_cross_fwd(CrossArgs p) {
 #pragma unroll
         for (int db = 0; db < DB; ++db) acc[db][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    keys.walk(p, [&](int64_t tile) {
+    auto use = [&](int64_t tile, auto part) __attribute__((always_inline)) {
         const unsigned char *const lk = keys.keys(tile), *const lv = keys.values(tile);
         f32x4 s[NB][R];
 #pragma unroll
@@ -159,23 +171,18 @@ __global__ __launch_bounds__(256) void k_cross_fwd(CrossArgs p) {
                 for (int i = 0; i < R; ++i) s[nb][i] = mma<T>(a, qf[i][ks], s[nb][i]);
             }
         }
-        if (keys.mask) {
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                const uint32_t w = *(const uint32_t*)(keys.seen(tile) + wk * KW + nb * 16 + 4 * g);
-#pragma unroll
-                for (int i = 0; i < R; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s[nb][i][e] = (w >> (8 * e)) & 0xff ? s[nb][i][e] : kNegInf;
-            }
-        } else if ((tile + 1) * TK > keys.len) {
+        if constexpr (part.value) {
             const int left = keys.left(tile) - wk * KW - 4 * g;
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
+            for (int nb = 0; nb < NB; ++nb) {
+                const uint32_t w = keys.mask ? *(const uint32_t*)(keys.seen(tile) + wk * KW + nb * 16 + 4 * g) : 0x01010101u;
 #pragma unroll
-                for (int i = 0; i < R; ++i)
+                for (int e = 0; e < 4; ++e) {
+                    const bool in = nb * 16 + e < left && ((w >> (8 * e)) & 0xff);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[nb][i][e] = nb * 16 + e < left ? s[nb][i][e] : kNegInf;
+                    for (int i = 0; i < R; ++i) s[nb][i][e] = in ? s[nb][i][e] : kNegInf;
+                }
+            }
         }
 #pragma unroll
         for (int i = 0; i < R; ++i) {
@@ -184,15 +191,15 @@ __global__ __launch_bounds__(256) void k_cross_fwd(CrossArgs p) {
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[nb][i][e]);
-            mx = fmaxf(across_groups_max(mx), m[i]);
-            if (__any(mx > m[i])) {  // else the sums keep their scale
-                const float f = mx == kNegInf ? 1.f : __builtin_amdgcn_exp2f((m[i] - mx) * p.c);
-                m[i] = mx;
+            mx = across_groups_max(mx);
+            if (__any((mx - m[i]) * p.c > kSlack)) {
+                const float top = fmaxf(mx, m[i]), f = top == kNegInf ? 1.f : __builtin_amdgcn_exp2f((m[i] - top) * p.c);
+                m[i] = top;
                 l[i] *= f;
 #pragma unroll
                 for (int db = 0; db < DB; ++db) acc[db][i] *= f;
             }
-            const float mc = mx == kNegInf ? 0.f : mx * p.c;  // no key seen so far: every power is 0
+            const float mc = m[i] == kNegInf ? 0.f : m[i] * p.c;  // no key seen so far: every power is 0
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -213,7 +220,8 @@ __global__ __launch_bounds__(256) void k_cross_fwd(CrossArgs p) {
                 for (int i = 0; i < R; ++i) acc[db][i] = mma<T>(a, pf[i], acc[db][i]);
             }
         }
-    });
+    };
+    keys.walk(p, [&](int64_t t) { use(t, std::false_type()); }, [&](int64_t t) { use(t, std::true_type()); });
 #pragma unroll
     for (int i = 0; i < R; ++i) l[i] = across_groups_sum(l[i]);
 

@@ -164,6 +164,33 @@ __device__ __forceinline__ void store4(T* row, int c, int d, f32x4 v) {
     }
 }
 
+// A buffer from `base` (the same for the wave) on, as the builtins and as the
+// instruction take it. Loads check their rows themselves and give kOOB where
+// there is none; valid offsets are below 2^31.
+struct Buffer {
+    rsrc_t r;
+    u32x4 q;
+};
+__device__ __forceinline__ Buffer open_buffer(const void* base) {
+    const uint64_t at = (uint64_t)base;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)at), hi = __builtin_amdgcn_readfirstlane((uint32_t)(at >> 32));
+    return {make_rsrc(base, 0x7fffffffu), u32x4{lo, hi & 0xffffu, 0x7fffffffu, 0x00020000u}};
+}
+
+// 16 bytes per lane from `offset` in the buffer to 16 lane + `to` in LDS (`to` is
+// the same for the wave). Written as the instruction itself: before any read of
+// LDS the compiler waits for the loads to LDS that it knows of, as it cannot
+// tell which of two tiles they go to, and no load would be in flight during the
+// work on the tile before. There is no output register; `landed` waits.
+__device__ __forceinline__ void load_to_lds(u32x4 r, uint32_t offset, const unsigned char* to) {
+    typedef __attribute__((address_space(3))) const unsigned char* lds;
+    const uint32_t base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds)to);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :
+                 : "s"(base), "v"(offset), "s"(r)
+                 : "memory", "m0");
+}
+
 // One thread's share of loading a tile of TILE rows by W elements to LDS through
 // a buffer descriptor: rows that do not exist, and columns past d, arrive as
 // zeros without a branch. VEC: straight to LDS, without registers; a barrier
@@ -182,20 +209,18 @@ struct Stage {
     }
 
     // piece i, of a row that starts `at` bytes from the descriptor's (kOOB: none)
-    __device__ __forceinline__ void load(int i, rsrc_t r, uint32_t at, int d, unsigned char* tile) {
+    __device__ __forceinline__ void load(int i, const Buffer& r, uint32_t at, int d, unsigned char* tile) {
         constexpr int S = (int)sizeof(T);
         const int c = col(i);
         if constexpr (VEC) {
-            typedef __attribute__((address_space(3))) void* lds;
-            unsigned char* const to = tile + (i * 256 + (threadIdx.x & ~63)) * 16;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds)to, 16, c < d ? at + c * S : kOOB, 0, 0, 0);
+            load_to_lds(r.q, c < d ? at + c * S : kOOB, tile + (i * 256 + (threadIdx.x & ~63)) * 16);
         } else {
             Pack<T, E> p;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const uint32_t off = c + e < d ? at + (c + e) * S : kOOB;
-                if constexpr (S == 2) p.e[e] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0));
-                else p.e[e] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0));
+                if constexpr (S == 2) p.e[e] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(r.r, off, 0, 0));
+                else p.e[e] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(r.r, off, 0, 0));
             }
             v[i] = __builtin_bit_cast(u32x4, p);
         }
@@ -211,13 +236,6 @@ struct Stage {
 // Waits for this wave's loads to LDS (which the compiler does not wait for)
 __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
-// A descriptor from `base` on. Loads check their rows themselves and give kOOB
-// where there is none; valid offsets are below 2^31.
-template <typename T>
-__device__ __forceinline__ rsrc_t open_rsrc(const T* base) {
-    return make_rsrc(base, 0x7fffffffu);
-}
-
 // ---------------------------------------------------------------------------
 
 struct CrossArgs {
@@ -231,7 +249,7 @@ struct CrossArgs {
     int64_t qb, qn, qh, kb, kn, kh, vb, vn, vh, ob, on, oh, gb, gn, gh;  // element strides of q, k, v, o, dout
     int64_t mask_b, mask_n;
     int B, H, KH, G, D;    // G = H / KH query heads per key head
-    int64_t Nq, Nk, M;     // M = Nq G rows per key head: row r is query r / G, head (key head) G + r % G
+    int64_t Nq, Nk, M;     // M = Nq G rows per key head (below 2^31): row r is query r / G, head (key head) G + r % G
     int splits;            // of the reduced axis
     float c, scale;        // c = scale log2(e)
     float inv_g;           // 1 / G
@@ -244,22 +262,22 @@ struct CrossArgs {
 // load all XCDs alike. The heads beyond a multiple of 8 are cut across XCDs.
 struct HeadTile {
     int bh;
-    int64_t tile;
+    uint32_t tile;
 };
-__device__ __forceinline__ HeadTile head_tile(int64_t w, int64_t grid, int64_t n) {
-    const int64_t eights = grid / n / 8, whole = eights * 8 * n;
+__device__ __forceinline__ HeadTile head_tile(uint32_t w, uint32_t grid, uint32_t n) {
+    const uint32_t eights = grid / n / 8, whole = eights * 8 * n;
     if (w < whole) {
-        const int64_t k = w >> 3, q = k / n;
+        const uint32_t k = w >> 3, q = k / n;
         return {(int)(q * 8 + (w & 7)), k - q * n};
     }
-    const int64_t t = xcd_tile(w - whole, grid - whole), q = t / n;
+    const uint32_t t = (uint32_t)xcd_tile(w - whole, grid - whole), q = t / n;
     return {(int)(eights * 8 + q), t - q * n};
 }
 
 // Row r of the M rows of key head `j`: the offset of its query and head
 __device__ __forceinline__ int64_t row_at(const CrossArgs& p, int64_t r, int64_t sn, int64_t sh, int j) {
     if (p.G == 1) return r * sn + j * sh;
-    const uint64_t n = (uint64_t)r / (uint32_t)p.G;
+    const uint32_t n = (uint32_t)r / (uint32_t)p.G;
     return n * sn + (int64_t)(j * p.G + (int)(r - n * p.G)) * sh;
 }
 
@@ -271,7 +289,7 @@ struct RowTile {
 };
 __device__ __forceinline__ RowTile row_tile(const CrossArgs& p, int64_t r0) {
     if (p.G == 1) return {r0, 0};
-    const uint64_t n = (uint64_t)r0 / (uint32_t)p.G;
+    const uint32_t n = (uint32_t)r0 / (uint32_t)p.G;
     return {(int64_t)n, (int)(r0 - n * p.G)};
 }
 __device__ __forceinline__ uint32_t row_tile_at(const CrossArgs& p, const RowTile& t, int i, int64_t sn, int64_t sh, int size) {

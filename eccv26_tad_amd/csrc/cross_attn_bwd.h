@@ -55,7 +55,7 @@ __global__ __launch_bounds__(256) void k_cross_bwd_q(CrossArgs p) {
         }
         delta[i] = across_groups_sum(s);
         lse[i] = in ? p.lse[bh * p.M + r] : -kNegInf;
-        if (in && g == 0 && wk == 0 && split == 0) p.delta[bh * p.M + r] = delta[i];
+        if (in && g == 0 && wk == 0 && split == 0) p.delta[bh * p.M + r] = -delta[i];
     }
     if (!p.out) return;
 
@@ -204,10 +204,12 @@ __global__ __launch_bounds__(256) void k_cross_bwd_kv(CrossArgs p) {
             sq.load(i, rq, r < n ? row_tile_at(p, rt, r, p.qn, p.qh, sizeof(T)) : kOOB, p.D, mem[tile & 1][0]);
             sd.load(i, rd, r < n ? row_tile_at(p, rt, r, p.gn, p.gh, sizeof(T)) : kOOB, p.D, mem[tile & 1][1]);
         }
-        if (threadIdx.x < TQ) {
-            const int64_t r = tile * TQ + threadIdx.x;
-            ll[tile & 1][threadIdx.x] = r < p.M ? p.lse[bh * p.M + r] : -kNegInf;  // past the end: probabilities 0
-            lde[tile & 1][threadIdx.x] = r < p.M ? -p.delta[bh * p.M + r] : 0.f;
+        // Past the end zeros, as for the rows themselves: a probability of 1
+        // then meets a gradient of 0.
+        if (wave < 2) {
+            const uint32_t at = lane < n ? lane * 4 : kOOB;
+            if (wave == 0) load_word_to_lds(open_buffer(p.lse + bh * p.M + tile * TQ).q, at, ll[tile & 1]);
+            else load_word_to_lds(open_buffer(p.delta + bh * p.M + tile * TQ).q, at, lde[tile & 1]);
         }
     };
     auto arrive = [&](int64_t tile) {
@@ -220,11 +222,7 @@ __global__ __launch_bounds__(256) void k_cross_bwd_kv(CrossArgs p) {
     for (int i = 0; i < R; ++i)
 #pragma unroll
         for (int db = 0; db < DB; ++db) dk[db][i] = dv[db][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (t0 < t1) {
-        fetch(t0);
-        arrive(t0);
-    }
-    for (int64_t tile = t0; tile < t1; ++tile) {
+    auto use = [&](int64_t tile) __attribute__((always_inline)) {
         __syncthreads();
         if (tile + 1 < t1) fetch(tile + 1);
         const unsigned char *const lq = mem[tile & 1][0], *const ld = mem[tile & 1][1];
@@ -280,6 +278,11 @@ __global__ __launch_bounds__(256) void k_cross_bwd_kv(CrossArgs p) {
             }
         }
         if (tile + 1 < t1) arrive(tile + 1);
+    };
+    if (t0 < t1) {
+        fetch(t0);
+        arrive(t0);
+        for (int64_t tile = t0; tile < t1; ++tile) use(tile);
     }
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll

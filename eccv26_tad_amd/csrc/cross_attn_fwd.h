@@ -48,7 +48,7 @@ struct KeyTiles {
     unsigned char* mem;     // [kBuffers][K, V]
     uint8_t* seen_mem;      // [kBuffers][TK]
     uint8_t next[S::kCount];  // the mask at the next tile's rows
-    uint8_t own;              // and at row threadIdx.x
+    uint8_t own, own_next;    // and at row threadIdx.x
 
     __device__ __forceinline__ KeyTiles(const CrossArgs& p, int b, int j, int split, unsigned char* mem, uint8_t* seen_mem)
         : k((const T*)p.k + b * p.kb + j * p.kh), v((const T*)p.v + b * p.vb + j * p.vh),
@@ -71,20 +71,25 @@ struct KeyTiles {
         for (int i = 0; i < S::kCount; ++i) next[i] = S::row(i) < n ? m[S::row(i) * p.mask_n] : 0;
         own = (int)threadIdx.x < n ? m[threadIdx.x * p.mask_n] : 0;  // n is at most TK
     }
+    template <bool MASK>  // false: there is no mask
     __device__ __forceinline__ void fetch(const CrossArgs& p, int64_t tile) {
         const int n = left(tile);
         const Buffer rk = open_buffer(k + tile * TK * p.kn), rv = open_buffer(v + tile * TK * p.vn);
 #pragma unroll
         for (int i = 0; i < S::kCount; ++i) {
             const int r = S::row(i);
-            const bool in = r < n && (!mask || next[i]);
+            const bool in = r < n && (!MASK || !mask || next[i]);
             sk.load(i, rk, in ? (uint32_t)(r * (int)p.kn) * (int)sizeof(T) : kOOB, p.D, keys(tile));
             sv.load(i, rv, in ? (uint32_t)(r * (int)p.vn) * (int)sizeof(T) : kOOB, p.D, values(tile));
         }
-        if (mask && threadIdx.x < TK) seen(tile)[threadIdx.x] = own;
-        fetch_mask(p, tile + 1);
+        if constexpr (MASK) {
+            own_next = own;
+            fetch_mask(p, tile + 1);
+        }
     }
+    template <bool MASK>
     __device__ __forceinline__ void arrive(int64_t tile) {
+        if (MASK && mask && threadIdx.x < TK) seen(tile)[threadIdx.x] = own_next;
         sk.store(keys(tile));
         sv.store(values(tile));
         landed();
@@ -99,22 +104,22 @@ struct KeyTiles {
         const int64_t tw = mask ? t0 : max<int64_t>(t0, lesser(t1, len / TK));
         fetch_mask(p, t0);
         if constexpr (kBuffers == 2) {
-            fetch(p, t0);
-            arrive(t0);
+            fetch<true>(p, t0);
+            arrive<true>(t0);
         }
-        for (int64_t tile = t0; tile < tw; ++tile) step(p, tile, whole);
-        for (int64_t tile = tw; tile < t1; ++tile) step(p, tile, part);
+        for (int64_t tile = t0; tile < tw; ++tile) step<false>(p, tile, whole);
+        for (int64_t tile = tw; tile < t1; ++tile) step<true>(p, tile, part);
     }
-    template <typename F>
+    template <bool MASK, typename F>
     __device__ __forceinline__ void step(const CrossArgs& p, int64_t tile, F use) {
         __syncthreads();  // this tile has arrived, and nobody reads the other any more
         if constexpr (kBuffers == 2) {
-            if (tile + 1 < t1) fetch(p, tile + 1);
+            if (tile + 1 < t1) fetch<MASK>(p, tile + 1);
             use(tile);
-            if (tile + 1 < t1) arrive(tile + 1);
+            if (tile + 1 < t1) arrive<MASK>(tile + 1);
         } else {
-            fetch(p, tile);
-            arrive(tile);
+            fetch<MASK>(p, tile);
+            arrive<MASK>(tile);
             __syncthreads();
             use(tile);
         }

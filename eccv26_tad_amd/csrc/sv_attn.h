@@ -191,6 +191,16 @@ __device__ __forceinline__ void load_to_lds(u32x4 r, uint32_t offset, const unsi
                  : "memory", "m0");
 }
 
+// The same for 4 bytes per lane.
+__device__ __forceinline__ void load_word_to_lds(u32x4 r, uint32_t offset, const void* to) {
+    typedef __attribute__((address_space(3))) const unsigned char* lds;
+    const uint32_t base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds)to);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+                 :
+                 : "s"(base), "v"(offset), "s"(r)
+                 : "memory", "m0");
+}
+
 // One thread's share of loading a tile of TILE rows by W elements to LDS through
 // a buffer descriptor: rows that do not exist, and columns past d, arrive as
 // zeros without a branch. VEC: straight to LDS, without registers; a barrier
@@ -233,8 +243,15 @@ struct Stage {
     }
 };
 
-// Waits for this wave's loads to LDS (which the compiler does not wait for)
-__device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// Waits for this wave's loads to LDS (which the compiler does not know of), by
+// the builtin, from which the compiler sees that its own loads are done as well:
+// else it would wait for those made before a loop inside it, and with them for
+// the loads to LDS.
+__device__ __forceinline__ void landed() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    asm volatile("" ::: "memory");
+}
 
 // ---------------------------------------------------------------------------
 
@@ -242,7 +259,7 @@ struct CrossArgs {
     const void *q, *k, *v, *o, *dout;
     void *out, *dk, *dv;   // out: the forward's output, or dq
     float* lse;            // [B KH][M]: log2 of a row's sum of 2^(c s), +inf for a row that sees no key
-    float* delta;          // [B KH][M]: sum over d of dout out
+    float* delta;          // [B KH][M]: minus the sum over d of dout out
     const int32_t* lengths;   // [B] or NULL
     const uint8_t* mask;      // [B, Nk] by mask_b, mask_n, or NULL; nonzero: the key is seen
     float* part;           // partial results of the splits (NULL: none)

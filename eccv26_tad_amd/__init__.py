@@ -48,7 +48,7 @@ from .neighbor import (  # noqa: E402
 )
 from .adapter import (AdapterDownFunction, AdapterUpFunction, SparseConvAdapter,  # noqa: E402
                       SparseConvAdapterFunction)
-from .cross_attention import CrossAttention, CrossAttentionFunction, cross_attention  # noqa: E402
+from .cross_attention import CrossAttention, cross_attention  # noqa: E402
 from .dense_path import (  # noqa: E402
     conv2d_weight_from_sparse,
     dense_conv_tokens,
@@ -56,7 +56,7 @@ from .dense_path import (  # noqa: E402
     sparse_weight_from_conv2d,
 )
 from .grad_clip import clip_grad_norm_, clip_grads, grad_norm  # noqa: E402
-from .layer_norm import LayerNormFunction, layer_norm  # noqa: E402
+from .layer_norm import layer_norm  # noqa: E402
 from .sparse_conv_layer import (  # noqa: E402
     SparseConv2d,
     SparseConv2dFunction,
@@ -76,7 +76,7 @@ __all__ = [
     "remap_legacy_sparse_conv_weights",
     "dense_conv_tokens", "keep_mask_from_indices", "sparse_weight_from_conv2d",
     "conv2d_weight_from_sparse", "SparseConvAdapter", "AdapterDownFunction", "AdapterUpFunction", "SparseConvAdapterFunction",
-    "layer_norm", "LayerNormFunction", "cross_attention", "CrossAttention", "CrossAttentionFunction",
+    "layer_norm", "cross_attention", "CrossAttention",
     "clip_grads", "clip_grad_norm_", "grad_norm",
     "LIB_PATH",
 ]

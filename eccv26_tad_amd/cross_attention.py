@@ -11,32 +11,9 @@ import math
 
 import torch
 import torch.nn as nn
-from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import opentad_sparse_ops as _ops
 from .layer_norm import layer_norm
-
-
-class CrossAttentionFunction(Function):
-    """autograd node of ``cross_attention``; keeps the output and one float32
-    per row, from which the backward recomputes the probabilities."""
-
-    @staticmethod
-    def forward(ctx, q, k, v, key_lengths, key_mask, scale):
-        out, lse = _ops.cross_attention(q, k, v, key_lengths, key_mask, scale, True)
-        ctx.save_for_backward(q, k, v, out, lse, key_lengths, key_mask)
-        ctx.scale = scale
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout):
-        q, k, v, out, lse, key_lengths, key_mask = ctx.saved_tensors
-        need_q, need_k, need_v = ctx.needs_input_grad[:3]
-        dq, dk, dv = _ops.cross_attention_bwd(dout, q, k, v, out, lse, key_lengths, key_mask, ctx.scale, need_q,
-                                              need_k or need_v)
-        return dq, dk if need_k else None, dv if need_v else None, None, None, None
 
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_lengths: torch.Tensor | None = None,
@@ -61,7 +38,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_lengt
     if key_lengths is not None and key_lengths.dtype == torch.int64:
         key_lengths = key_lengths.clamp(0, k.shape[1]).to(torch.int32)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return CrossAttentionFunction.apply(q, k, v, key_lengths, key_mask, scale)
+        return _ops.cross_attention_grad(q, k, v, key_lengths, key_mask, scale)
     return _ops.cross_attention(q, k, v, key_lengths, key_mask, scale, False)[0]
 
 

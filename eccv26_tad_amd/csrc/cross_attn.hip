@@ -8,7 +8,7 @@ namespace svtad {
 
 constexpr int kMaxHeadDim = 128;
 constexpr int kWantGroups = 512;  // two workgroups per compute unit
-constexpr int kMaxSplits = 64;
+constexpr int kMaxSplits = 64;  // k_cross_join holds a quarter of them in registers
 
 // How a kernel over row tiles (forward, dq) is cut: waves along the rows, and
 // splits of the keys. Rows are not padded to more than twice their number where
@@ -31,7 +31,7 @@ static RowPlan row_plan(const svtad_cross_args& a) {
 // Splits of the rows in the kernel over key tiles.
 static int key_plan(const svtad_cross_args& a) {
     const int64_t m = a.nq * (a.heads / a.kv_heads);
-    const int64_t groups = std::max<int64_t>(1, cdiv(a.nk, cross_kv_keys(a.head_dim)) * a.batch * a.kv_heads);
+    const int64_t groups = std::max<int64_t>(1, cdiv(a.nk, kCrossKvKeys) * a.batch * a.kv_heads);
     return (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(kWantGroups, groups), cdiv(m, 64) / 2, (int64_t)kMaxSplits}));
 }
 
@@ -71,7 +71,7 @@ static int cross_check(const svtad_cross_args* a, int dtype) {
         return set_error(SVTAD_ERR_INVALID, "cross_attention: scale must be positive and finite");
     const double m = (double)a->nq * (a->heads / a->kv_heads), bk = (double)a->batch * a->kv_heads;
     if ((m / 16 + 1) * bk * kMaxSplits > INT32_MAX || ((double)a->nk / 64 + 1) * bk * kMaxSplits > INT32_MAX ||
-        bk * std::max(m, (double)a->nk) * 64 > (double)INT32_MAX * 256)
+        bk * std::max(m, (double)a->nk) * 64 > (double)INT32_MAX * 64)
         return set_error(SVTAD_ERR_UNSUPPORTED, "cross_attention: too many rows or keys for one launch");
     const int g = a->heads / a->kv_heads;
     if (!near_strides(a->q_stride, g, dtype) || !near_strides(a->k_stride, 1, dtype) || !near_strides(a->v_stride, 1, dtype))

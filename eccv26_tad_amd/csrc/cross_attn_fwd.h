@@ -2,22 +2,19 @@
 //
 //   s = scale q . k,  p = softmax of s over the seen keys,  out = sum p v
 //
-// One pass over the keys with each row's running maximum and sum (float32).
-// A workgroup of 4 waves owns WM R 16 rows of one key head (R row tiles of 16
-// per wave) and walks over key tiles staged in LDS, the next tile's loads in
-// flight in registers meanwhile; with WM < 4 the waves of equal rows share a
-// tile's keys and are joined at the end. Rows are queries times the G query
-// heads of the key head, so shared key heads are read once for all of them.
-// With few rows the keys are split over workgroups, whose partial sums
-// k_cross_join adds in a fixed order.
+// One pass over the keys with each row's running scale and sum (float32). A
+// workgroup of 4 waves owns WM S rows of one key head (S rows per wave) and walks
+// over key tiles staged in LDS, the next tile's loads in flight meanwhile; with
+// WM < 4 the waves of equal rows share a tile's keys and are joined at the end.
+// Rows are queries times the G query heads of the key head, so shared key heads
+// are read once for all of them. With few rows the keys are split over
+// workgroups, whose partial sums k_cross_join adds in a fixed order.
 //
 // Probabilities are rounded to T for the product with v (the matrix units'
-// operand type); their sum, the maximum and the output's sums stay float32.
+// operand type); their sum, the scale and the output's sums stay float32.
 // Keys that are not seen are staged as zeros and their scores replaced, so
 // neither infinities nor NaN in their places reach a result.
 #pragma once
-
-#include <type_traits>
 
 #include "cross_attn.h"
 
@@ -25,10 +22,13 @@ namespace svtad {
 
 constexpr float kNegInf = -__builtin_huge_valf();
 
-// The sums keep the scale of an earlier maximum until a score is 2^kSlack above
-// it: after the first tiles of a row they are hardly rescaled again (32 products
-// per tile and lane otherwise), and the powers stay below 2^kSlack.
-constexpr float kSlack = 8.f;
+// A row's powers are taken relative to the largest score seen when its scale was
+// last set. The scale is set again only when a lane's powers of one tile add up
+// to more than kLimit: the tile is then computed a second time with its maximum.
+// Otherwise no tile needs a maximum, whose cost per score is a third of the
+// exponential's, nor the sums a rescaling; float32 sums and the operand types
+// hold powers of that size as well as those below 1.
+constexpr float kLimit = 4096.f;
 
 // Keys of a staged tile: 64, or 32 per wave where the waves share a tile.
 template <int WM> constexpr int kTileKeys = WM == 1 ? 128 : 64;
@@ -126,194 +126,210 @@ struct KeyTiles {
     }
 };
 
-template <typename T, int DP, int WM, int R, bool VEC>
-__global__ __launch_bounds__(256) void k_cross_fwd(CrossArgs p) {
-    constexpr int W = DP < 32 ? 32 : DP, KS = W / 32, DB = DP / 16;
-    constexpr int WK = 4 / WM, TK = kTileKeys<WM>, KW = TK / WK, NB = KW / 16, ROWS = WM * R * 16;
-    static_assert(KW % 32 == 0, "a wave's keys fill whole products");
-    typedef LdsTile<T, W> Tile;
+template <typename T, int DP, int WM, int S, bool VEC>
+__global__ __launch_bounds__(256, (kResidentFwd<T, DP>)) void k_cross_fwd(CrossArgs p) {
+    typedef Shape<T, S> M;
+    typedef typename M::Acc Acc;
+    constexpr int W = DP < 32 ? 32 : DP, KS = W / M::K, DB = DP < S ? 1 : DP / S;
+    constexpr int WK = 4 / WM, TK = kTileKeys<WM>, KW = TK / WK, NB = KW / S, ROWS = WM * S;
     typedef KeyTiles<T, TK, W, VEC> Keys;
-    constexpr size_t kJoin = WK > 1 ? (size_t)WK * ROWS * (DP + 2) * 4 : 0;
+    constexpr size_t kJoin = WK > 1 ? (size_t)WK * ROWS * (DB * S + 2) * 4 : 0;
     __shared__ __attribute__((aligned(16))) unsigned char mem[Keys::kBytes > kJoin ? Keys::kBytes : kJoin];
     __shared__ __attribute__((aligned(16))) uint8_t seen_mem[Keys::kBuffers * TK];
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave % WM, wk = wave / WM;
-    const int g = lane >> 4, li = lane & 15;
+    const int li = M::col(lane), slot = M::slot(lane);
     const uint32_t row_tiles = ((uint32_t)p.M + ROWS - 1) / ROWS;
     const HeadTile ht = head_tile(blockIdx.x, gridDim.x, row_tiles * p.splits);
-    const int bh = ht.bh, b = bh / p.KH, j = bh - b * p.KH, split = (int)(ht.tile / row_tiles);
-    const int64_t r0 = (int64_t)(ht.tile - split * row_tiles) * ROWS;
+    const int j = ht.bh % p.KH, b = sample_of_rank(p, ht.bh / p.KH), bh = b * p.KH + j, split = (int)(ht.tile / row_tiles);
+    const int64_t r = (int64_t)(ht.tile - split * row_tiles) * ROWS + wm * S + li;  // this lane's row
     Keys keys(p, b, j, split, mem, seen_mem);
 
-    Frag8<T> qf[R][KS];
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const int64_t r = r0 + (wm * R + i) * 16 + li;
+    Frag8<T> qf[KS];
+    {
         const T* const q = (const T*)p.q + b * p.qb + (r < p.M ? row_at(p, r, p.qn, p.qh, j) : 0);
 #pragma unroll
-        for (int s = 0; s < KS; ++s) qf[i][s] = load_frag<T, VEC>(q, s * 32 + g * 8, r < p.M ? p.D : 0);
+        for (int s = 0; s < KS; ++s) qf[s] = load_frag<T, VEC>(q, s * M::K + slot * 8, r < p.M ? p.D : 0);
     }
-
-    f32x4 acc[DB][R];
-    float m[R], l[R];
+    Acc acc[DB];
+    float m = kNegInf, l = 0.f;
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        m[i] = kNegInf, l[i] = 0.f;
-#pragma unroll
-        for (int db = 0; db < DB; ++db) acc[db][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
+    for (int db = 0; db < DB; ++db) acc[db] = M::fill(0.f);
     auto use = [&](int64_t tile, auto part) __attribute__((always_inline)) {
         const unsigned char *const lk = keys.keys(tile), *const lv = keys.values(tile);
-        f32x4 s[NB][R];
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-            for (int i = 0; i < R; ++i) s[nb][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const Frag8<T> a = Tile::frag(lk, wk * KW + nb * 16, ks, lane);
-#pragma unroll
-                for (int i = 0; i < R; ++i) s[nb][i] = mma<T>(a, qf[i][ks], s[nb][i]);
-            }
-        }
-        if constexpr (part.value) {
-            const int left = keys.left(tile) - wk * KW - 4 * g;
+        Acc s[NB];
+        float sum;
+        for (bool with_max = __any(m == kNegInf);; with_max = true) {
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-                const uint32_t w = keys.mask ? *(const uint32_t*)(keys.seen(tile) + wk * KW + nb * 16 + 4 * g) : 0x01010101u;
+                s[nb] = M::fill(0.f);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const bool in = nb * 16 + e < left && ((w >> (8 * e)) & 0xff);
-#pragma unroll
-                    for (int i = 0; i < R; ++i) s[nb][i][e] = in ? s[nb][i][e] : kNegInf;
-                }
+                for (int ks = 0; ks < KS; ++ks)
+                    s[nb] = M::mma(M::template frag<W>(lk, wk * KW + nb * S, ks, lane), qf[ks], s[nb]);
             }
-        }
+            if constexpr (part.value) {
+                const int left = keys.left(tile);
 #pragma unroll
-        for (int i = 0; i < R; ++i) {
-            float mx = s[0][i][0];
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int q = 0; q < M::Q; ++q) {
+                        const int at = wk * KW + nb * S + M::row4(q, lane);
+                        const uint32_t w = keys.mask ? *(const uint32_t*)(keys.seen(tile) + at) : 0x01010101u;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            s[nb][4 * q + e] = at + e < left && ((w >> (8 * e)) & 0xff) ? s[nb][4 * q + e] : kNegInf;
+                    }
+            }
+            if (with_max) {
+                float top = m;
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int e = 0; e < 4 * M::Q; ++e) top = fmaxf(top, s[nb][e]);
+                top = M::col_max(top);
+                const float f = top == kNegInf ? 1.f : __builtin_amdgcn_exp2f((m - top) * p.c);
+                m = top;
+                l *= f;
+#pragma unroll
+                for (int db = 0; db < DB; ++db) acc[db] *= f;
+            }
+            const float mc = m == kNegInf ? 0.f : m * p.c;  // no key seen so far: every power is 0
+            sum = 0.f;
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[nb][i][e]);
-            mx = across_groups_max(mx);
-            if (__any((mx - m[i]) * p.c > kSlack)) {
-                const float top = fmaxf(mx, m[i]), f = top == kNegInf ? 1.f : __builtin_amdgcn_exp2f((m[i] - top) * p.c);
-                m[i] = top;
-                l[i] *= f;
-#pragma unroll
-                for (int db = 0; db < DB; ++db) acc[db][i] *= f;
-            }
-            const float mc = m[i] == kNegInf ? 0.f : m[i] * p.c;  // no key seen so far: every power is 0
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    s[nb][i][e] = __builtin_amdgcn_exp2f(fmaf(s[nb][i][e], p.c, -mc));
-                    l[i] += s[nb][i][e];
+                for (int e = 0; e < 4 * M::Q; ++e) {
+                    s[nb][e] = __builtin_amdgcn_exp2f(fmaf(s[nb][e], p.c, -mc));
+                    sum += s[nb][e];
                 }
+            if (with_max || !__any(!(sum <= kLimit))) break;
         }
+        l += sum;
 #pragma unroll
-        for (int kg = 0; kg < NB / 2; ++kg) {
-            Frag8<T> pf[R];
+        for (int kk = 0; kk < KW / M::K; ++kk) {
+            const Frag8<T> pf = M::pack(s, kk);
 #pragma unroll
-            for (int i = 0; i < R; ++i) pf[i] = pack_frag<T>(s[2 * kg][i], s[2 * kg + 1][i]);
-#pragma unroll
-            for (int db = 0; db < DB; ++db) {
-                const Frag8<T> a = Tile::frag_t(lv, wk * KW + kg * 32, db, lane);
-#pragma unroll
-                for (int i = 0; i < R; ++i) acc[db][i] = mma<T>(a, pf[i], acc[db][i]);
-            }
+            for (int db = 0; db < DB; ++db)
+                acc[db] = M::mma(M::template frag_t<W>(lv, wk * KW + kk * M::K, db, lane), pf, acc[db]);
         }
     };
     keys.walk(p, [&](int64_t t) { use(t, std::false_type()); }, [&](int64_t t) { use(t, std::true_type()); });
-#pragma unroll
-    for (int i = 0; i < R; ++i) l[i] = across_groups_sum(l[i]);
+    l = M::col_sum(l);
 
     if constexpr (WK > 1) {  // join the waves of equal rows, in order
-        float* const jo = (float*)mem;               // [WK][ROWS][DP]
-        float* const jm = jo + WK * ROWS * DP;       // [WK][ROWS][2]
+        constexpr int DA = DB * S;
+        float* const jo = (float*)mem;            // [WK][ROWS][DA]
+        float* const jm = jo + WK * ROWS * DA;    // [WK][ROWS][2]
+        const int at = wm * S + li;
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-            const int r = (wm * R + i) * 16 + li;
-            if (g == 0) {
-                jm[(wk * ROWS + r) * 2] = m[i];
-                jm[(wk * ROWS + r) * 2 + 1] = l[i];
-            }
-#pragma unroll
-            for (int db = 0; db < DB; ++db) *(f32x4*)(jo + (wk * ROWS + r) * DP + db * 16 + 4 * g) = acc[db][i];
+        if (slot == 0) {
+            jm[(wk * ROWS + at) * 2] = m;
+            jm[(wk * ROWS + at) * 2 + 1] = l;
         }
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int q = 0; q < M::Q; ++q)
+                *(f32x4*)(jo + (wk * ROWS + at) * DA + db * S + M::row4(q, lane)) = M::quad(acc[db], q);
         __syncthreads();
         if (wk != 0) return;
+        float top = m;
 #pragma unroll
-        for (int i = 0; i < R; ++i) {
-            const int r = (wm * R + i) * 16 + li;
-            float top = m[i];
+        for (int w = 1; w < WK; ++w) top = fmaxf(top, jm[(w * ROWS + at) * 2]);
+        if (top != kNegInf) {
+            float f = __builtin_amdgcn_exp2f((m - top) * p.c);
+            l *= f;
 #pragma unroll
-            for (int w = 1; w < WK; ++w) top = fmaxf(top, jm[(w * ROWS + r) * 2]);
-            if (top == kNegInf) continue;
-            float f = __builtin_amdgcn_exp2f((m[i] - top) * p.c);
-            l[i] *= f;
-#pragma unroll
-            for (int db = 0; db < DB; ++db) acc[db][i] *= f;
+            for (int db = 0; db < DB; ++db) acc[db] *= f;
 #pragma unroll
             for (int w = 1; w < WK; ++w) {
-                f = __builtin_amdgcn_exp2f((jm[(w * ROWS + r) * 2] - top) * p.c);
-                l[i] += f * jm[(w * ROWS + r) * 2 + 1];
+                f = __builtin_amdgcn_exp2f((jm[(w * ROWS + at) * 2] - top) * p.c);
+                l += f * jm[(w * ROWS + at) * 2 + 1];
 #pragma unroll
-                for (int db = 0; db < DB; ++db) acc[db][i] += *(const f32x4*)(jo + (w * ROWS + r) * DP + db * 16 + 4 * g) * f;
+                for (int db = 0; db < DB; ++db)
+#pragma unroll
+                    for (int q = 0; q < M::Q; ++q) {
+                        const f32x4 v = *(const f32x4*)(jo + (w * ROWS + at) * DA + db * S + M::row4(q, lane));
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[db][4 * q + e] += v[e] * f;
+                    }
             }
-            m[i] = top;
+            m = top;
         }
     }
 
+    if (r >= p.M) return;
+    if (p.splits > 1) {
+        const int64_t at = ((int64_t)split * p.B * p.KH + bh) * p.M + r;
+        const int dp = (p.D + 3) & ~3;
+        float* const po = p.part + at * dp;
+        float* const pm = p.part + (int64_t)p.splits * p.B * p.KH * p.M * dp + at * 2;
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const int64_t r = r0 + (wm * R + i) * 16 + li;
-        if (r >= p.M) continue;
-        if (p.splits > 1) {
-            const int64_t at = ((int64_t)split * p.B * p.KH + bh) * p.M + r;
-            const int dp = (p.D + 3) & ~3;
-            float* const po = p.part + at * dp;
-            float* const pm = p.part + (int64_t)p.splits * p.B * p.KH * p.M * dp + at * 2;
+        for (int db = 0; db < DB; ++db)
 #pragma unroll
-            for (int db = 0; db < DB; ++db)
-                if (db * 16 + 4 * g < p.D) *(f32x4*)(po + db * 16 + 4 * g) = acc[db][i];
-            if (g == 0) {
-                pm[0] = m[i];
-                pm[1] = l[i];
+            for (int q = 0; q < M::Q; ++q) {
+                const int c = db * S + M::row4(q, lane);
+                if (c < p.D) *(f32x4*)(po + c) = M::quad(acc[db], q);
             }
-            continue;
+        if (slot == 0) {
+            pm[0] = m;
+            pm[1] = l;
         }
-        T* const o = (T*)p.out + (int64_t)b * p.Nq * p.H * p.D + row_at(p, r, (int64_t)p.H * p.D, p.D, j);
-        const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
-#pragma unroll
-        for (int db = 0; db < DB; ++db) store4<T>(o, db * 16 + 4 * g, p.D, acc[db][i] * inv);
-        if (p.lse && g == 0)
-            p.lse[bh * p.M + r] = l[i] == 0.f ? -kNegInf : m[i] * p.c + __builtin_amdgcn_logf(l[i]);
+        return;
     }
+    T* const o = (T*)p.out + (int64_t)b * p.Nq * p.H * p.D + row_at(p, r, (int64_t)p.H * p.D, p.D, j);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int q = 0; q < M::Q; ++q) store4<T>(o, db * S + M::row4(q, lane), p.D, M::quad(acc[db], q) * inv);
+    if (p.lse && slot == 0) p.lse[bh * p.M + r] = l == 0.f ? -kNegInf : m * p.c + __builtin_amdgcn_logf(l);
 }
 
-// The splits of a row joined in order: one thread per 4 output values.
+// The splits of a row joined in order, a chunk of 4 output values per thread of
+// each group
 template <typename T>
 __global__ __launch_bounds__(256) void k_cross_join(CrossArgs p) {
-    const int dp = (p.D + 3) & ~3, nd = dp / 4;
-    const int64_t rows = (int64_t)p.B * p.KH * p.M, e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (e >= rows * nd) return;
-    const int64_t at = e / nd;
-    const int c = (int)(e - at * nd) * 4;
-    const float* const pm = p.part + (int64_t)p.splits * rows * dp;
-    float top = kNegInf;
-    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, pm[(s * rows + at) * 2]);
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    float l = 0.f;
-    if (top != kNegInf)
-        for (int s = 0; s < p.splits; ++s) {
-            const float f = __builtin_amdgcn_exp2f((pm[(s * rows + at) * 2] - top) * p.c);
-            l += f * pm[(s * rows + at) * 2 + 1];
-            acc += *(const f32x4*)(p.part + (s * rows + at) * dp + c) * f;
+    __shared__ float red[kJoinGroups][64][2];
+    const int dp = (p.D + 3) & ~3, nd = dp / 4, chunk = threadIdx.x & 63, g = threadIdx.x >> 6;
+    const int64_t rows = (int64_t)p.B * p.KH * p.M, e = (int64_t)blockIdx.x * 64 + chunk;
+    const bool in = e < rows * nd;
+    const int64_t at = in ? e / nd : 0;
+    const int c = in ? (int)(e - at * nd) * 4 : 0;
+    const int per = (p.splits + kJoinGroups - 1) / kJoinGroups, s0 = lesser(p.splits, g * per), s1 = lesser(p.splits, s0 + per);
+    const float* const pm = p.part + (int64_t)p.splits * rows * dp + at * 2;
+    const float* const po = p.part + at * dp + c;
+    constexpr int kMost = 64 / kJoinGroups;  // splits of a group
+    float m[kMost], w[kMost], top = kNegInf, l = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f}, v[kMost];
+#pragma unroll
+    for (int i = 0; i < kMost; ++i)
+        if (s0 + i < s1) {  // uniform
+            m[i] = pm[(s0 + i) * rows * 2];
+            w[i] = pm[(s0 + i) * rows * 2 + 1];
+            v[i] = *(const f32x4*)(po + (s0 + i) * rows * dp);
         }
+#pragma unroll
+    for (int i = 0; i < kMost; ++i)
+        if (s0 + i < s1) top = fmaxf(top, m[i]);
+    red[g][chunk][0] = top;
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < kJoinGroups; ++q) top = fmaxf(top, red[q][chunk][0]);
+    if (top != kNegInf) {
+#pragma unroll
+        for (int i = 0; i < kMost; ++i)
+            if (s0 + i < s1) {
+                const float f = __builtin_amdgcn_exp2f((m[i] - top) * p.c);
+                l += f * w[i];
+                acc += v[i] * f;
+            }
+    }
+    red[g][chunk][1] = l;
+    acc = join_groups(acc, g, chunk);  // its barrier covers red
+    if (g != 0 || !in) return;
+#pragma unroll
+    for (int q = 1; q < kJoinGroups; ++q) l += red[q][chunk][1];
     const int64_t bh = at / p.M, r = at - bh * p.M, b = bh / p.KH;
     const int j = (int)(bh - b * p.KH);
     T* const o = (T*)p.out + b * p.Nq * p.H * p.D + row_at(p, r, (int64_t)p.H * p.D, p.D, j);
@@ -321,26 +337,25 @@ __global__ __launch_bounds__(256) void k_cross_join(CrossArgs p) {
     if (p.lse && c == 0) p.lse[at] = l == 0.f ? -kNegInf : top * p.c + __builtin_amdgcn_logf(l);
 }
 
-template <typename T, int WM, int R>
+template <typename T, int WM, int S>
 static void launch_cross_fwd(const CrossArgs& p, hipStream_t st) {
-    const unsigned grid = (unsigned)(cdiv(p.M, WM * R * 16) * p.B * p.KH * p.splits);
+    const unsigned grid = (unsigned)(cdiv(p.M, WM * S) * p.B * p.KH * p.splits);
     if (!p.vec) {
-        if (p.D <= 32) k_cross_fwd<T, 32, WM, R, false><<<grid, 256, 0, st>>>(p);
-        else k_cross_fwd<T, 128, WM, R, false><<<grid, 256, 0, st>>>(p);
-    } else if (p.D <= 16) k_cross_fwd<T, 16, WM, R, true><<<grid, 256, 0, st>>>(p);
-    else if (p.D <= 32) k_cross_fwd<T, 32, WM, R, true><<<grid, 256, 0, st>>>(p);
-    else if (p.D <= 64) k_cross_fwd<T, 64, WM, R, true><<<grid, 256, 0, st>>>(p);
-    else k_cross_fwd<T, 128, WM, R, true><<<grid, 256, 0, st>>>(p);
+        if (p.D <= 32) k_cross_fwd<T, 32, WM, S, false><<<grid, 256, 0, st>>>(p);
+        else k_cross_fwd<T, 128, WM, S, false><<<grid, 256, 0, st>>>(p);
+    } else if (p.D <= 32) k_cross_fwd<T, 32, WM, S, true><<<grid, 256, 0, st>>>(p);
+    else if (p.D <= 64) k_cross_fwd<T, 64, WM, S, true><<<grid, 256, 0, st>>>(p);
+    else k_cross_fwd<T, 128, WM, S, true><<<grid, 256, 0, st>>>(p);
 }
 
 template <typename T>
 void cross_fwd(const CrossArgs& p, int wave_rows, hipStream_t st) {
-    if (wave_rows == 4) launch_cross_fwd<T, 4, 2>(p, st);
-    else if (wave_rows == 2) launch_cross_fwd<T, 2, 2>(p, st);
-    else launch_cross_fwd<T, 1, 1>(p, st);
+    if (wave_rows == 4) launch_cross_fwd<T, 4, 32>(p, st);
+    else if (wave_rows == 2) launch_cross_fwd<T, 2, 32>(p, st);
+    else launch_cross_fwd<T, 1, 16>(p, st);
     if (p.splits > 1) {
         const int64_t n = (int64_t)p.B * p.KH * p.M * ((p.D + 3) / 4);
-        k_cross_join<T><<<(unsigned)cdiv(n, 256), 256, 0, st>>>(p);
+        k_cross_join<T><<<(unsigned)cdiv(n, 64), 256, 0, st>>>(p);
     }
 }
 

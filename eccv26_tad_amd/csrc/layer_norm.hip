@@ -237,25 +237,33 @@ __global__ __launch_bounds__(256) void k_layer_norm_bwd(LnArgs p) {
     }
 }
 
-// dw, db: the partial sums of all workgroups added in a fixed order (each of
-// 16 thread groups every 16th of them, then the groups), one rounding
+// dw, db: the partial sums of all workgroups added in a fixed order (32 thread
+// groups take consecutive shares of them, then the groups), one rounding. A
+// workgroup owns 32 sums, 8 lanes of 4 each.
 template <typename P>
 __global__ __launch_bounds__(256) void k_layer_norm_sum(const float* __restrict__ part, int groups, int c,
                                                         P* __restrict__ dw, P* __restrict__ db) {
-    __shared__ float red[16][17];
-    const int lane = threadIdx.x & 15, g = threadIdx.x >> 4;
-    const int e = blockIdx.x * 16 + lane;
-    float s = 0.f;
-    if (e < 2 * c)
-        for (int q = g; q < groups; q += 16) s += part[(int64_t)q * 2 * c + e];
-    red[g][lane] = s;
-    __syncthreads();
-    if (g != 0 || e >= 2 * c) return;
-    s = 0.f;
+    __shared__ float red[32][33];
+    const int lane = threadIdx.x & 7, g = threadIdx.x >> 3;
+    const int e = blockIdx.x * 32 + lane * 4;
+    const int per = (groups + 31) / 32, g0 = min(groups, g * per), n = min(groups, g0 + per) - g0;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    if (e + 4 <= 2 * c) {
+        add_strided(s, part + (int64_t)g0 * 2 * c + e, 2 * c, n);
+    } else {
+        for (int q = g0; q < g0 + n; ++q)
+            for (int k = 0; k < 4; ++k) s[k] += e + k < 2 * c ? part[(int64_t)q * 2 * c + e + k] : 0.f;
+    }
 #pragma unroll
-    for (int q = 0; q < 16; ++q) s += red[q][lane];
-    P* const to = e < c ? dw : db;
-    if (to) to[e < c ? e : e - c] = (P)s;
+    for (int k = 0; k < 4; ++k) red[g][lane * 4 + k] = s[k];
+    __syncthreads();
+    const int o = blockIdx.x * 32 + threadIdx.x;
+    if (threadIdx.x >= 32 || o >= 2 * c) return;
+    float v = 0.f;
+#pragma unroll
+    for (int q = 0; q < 32; ++q) v += red[q][threadIdx.x];
+    P* const to = o < c ? dw : db;
+    if (to) to[o < c ? o : o - c] = (P)v;
 }
 
 // ---------------------------------------------------------------------------
@@ -386,7 +394,7 @@ extern "C" int svtad_norm_bwd(const svtad_norm_args* p, const void* dy, void* dx
         if (dx || sums) ln_launch(a, true, s, dtype, grid, hs);
     }
     if (sums) {  // no row: zeros
-        const int blocks = (int)cdiv(2 * a.c, 16);
+        const int blocks = (int)cdiv(2 * a.c, 32);
         const float* part = (const float*)workspace;
         if (a.p32 || dtype == SVTAD_F32) k_layer_norm_sum<float><<<blocks, 256, 0, hs>>>(part, grid, a.c, (float*)dw, (float*)db);
         else if (dtype == SVTAD_F16) k_layer_norm_sum<f16><<<blocks, 256, 0, hs>>>(part, grid, a.c, (f16*)dw, (f16*)db);

@@ -1,16 +1,15 @@
 // Pieces shared by the cross-attention kernels (gfx950).
 //
-// All products run on 16 x 16 matrix-core tiles whose left operand comes from
-// LDS and whose right operand is in registers. A score tile is computed
-// transposed, S^T = K Q^T: each lane then holds scores of ONE query (lane %
-// 16) for 4 consecutive keys per tile, so the softmax runs in the lane (two
-// lane exchanges join the 4 lane groups), and the tile is, without any
-// movement, the right operand of the next product O^T = V^T P^T. That
-// product's 32 reduction values are the keys of two score tiles: lane group g
-// holds keys 4g .. 4g+3 of each, and V^T's operand is read to match, as two
-// transposing LDS reads of 4 keys. The backward kernels use the same two
-// patterns.
+// All products run on the matrix cores with the left operand from LDS and the
+// right operand in registers. A score tile is computed transposed, S^T = K Q^T:
+// each lane then holds scores of ONE query (lane % S, tiles of S x S, S 32 or
+// 16), so that the softmax runs in the lane and a row's sum takes one or two
+// lane exchanges, and the tile is, without any movement, the right operand of
+// the next product O^T = V^T P^T: V^T is read from LDS in the order in which
+// the lanes hold the keys. The backward kernels use the same two patterns.
 #pragma once
+
+#include <type_traits>
 
 #include "sv_internal.h"
 #include "sv_mfma.h"
@@ -23,9 +22,7 @@ __device__ __forceinline__ I lesser(I a, I b) {  // in integers (an overloaded m
     return a < b ? a : b;
 }
 
-// 8 reduction values of a 16 x 16 x 32 product per lane; float32 runs it as
-// eight 16 x 16 x 4 products, whose operands pair values of equal position, so
-// the same layout serves.
+// 8 reduction values of a product, per lane
 template <typename T> struct Frag8 {
     T e[8] __attribute__((aligned(16)));
 };
@@ -35,17 +32,6 @@ template <> struct Frag8<f16> {
 template <> struct Frag8<bf16> {
     u32x4 v;
 };
-
-template <typename T>
-__device__ __forceinline__ f32x4 mma(const Frag8<T>& a, const Frag8<T>& b, f32x4 c) {
-    if constexpr (sizeof(T) == 2) {
-        return MfmaOp<T>::run(a.v, b.v, c);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.e[j], b.e[j], c, 0, 0, 0);
-        return c;
-    }
-}
 
 template <typename T> __device__ __forceinline__ Frag8<T> zero_frag() {
     return __builtin_bit_cast(Frag8<T>, Pack<T, 8>{});
@@ -65,89 +51,144 @@ __device__ __forceinline__ Frag8<T> load_frag(const T* row, int c, int d) {
     }
 }
 
-// The right operand of a 32-value product from two score tiles of a lane
-typedef float f32x8 __attribute__((ext_vector_type(8)));
-template <typename T>
-__device__ __forceinline__ Frag8<T> pack_frag(const f32x4& a, const f32x4& b) {
-    typedef T tx8 __attribute__((ext_vector_type(8)));
-    const f32x8 v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-    return __builtin_bit_cast(Frag8<T>, __builtin_convertvector(v, tx8));
-}
-
 // A tile of rows of W elements in LDS, in pieces of 16 bytes without padding
 // (so that a wave's loads may land there directly, 64 consecutive pieces at a
 // time). Row r keeps its piece c at place c ^ swizzle(r), which spreads both
-// kinds of reads over all banks: the same piece of 16 rows (frag), and two
-// neighbouring pieces of 8 rows (frag_t), whose swizzles differ above bit 0.
+// kinds of reads over all banks: the same piece of 16 rows (frag), and 2 or 4
+// neighbouring pieces of 8 or 4 rows (frag_t). For both the swizzle is the row's
+// number, in units of the rows that fill all banks (256 bytes), with its bits
+// reversed: neighbouring rows differ in the highest bit.
 template <typename T, int W>
 struct LdsTile {
     static constexpr int kRow = W * (int)sizeof(T), kPieces = kRow / 16, kElems = 16 / (int)sizeof(T);
     static constexpr int kBits = kRow >= 256 ? 4 : kRow == 128 ? 3 : 2, kShift = 4 - kBits;
 
     static __device__ __forceinline__ int swizzle(int r) {
-        const int e = (r & 15) >> kShift;
-        return ((e << 1) | (e >> (kBits - 1))) & ((1 << kBits) - 1);
+        return (int)(__builtin_bitreverse32((uint32_t)((r & 15) >> kShift)) >> (32 - kBits));
     }
-    // 8 elements ks * 32 + 8 (lane / 16) .. of row r0 + lane % 16; r0 a multiple of 16
+};
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// Products of S x S tiles, 64 lanes: lane l has column l % S of the right operand
+// and of the result and row l % S of the left one, with 8 reduction values at
+// slot l / S of K = 512 / S. Its 4 Q result values are rows row4(q) .. + 3 of
+// group q. float32 runs as eight products whose operands pair values of equal
+// position, so the same layout serves. S 32 takes fewer operand reads per
+// product and more issue slots are free beside it (random operands, one or two
+// waves per SIMD: 1850 TFLOP/s against 1150 and 1540 with S 16); S 16 wastes
+// less on a few rows.
+template <typename T, int S>
+struct Shape {
+    typedef float Acc __attribute__((ext_vector_type(S * S / 64)));
+    static constexpr int K = 512 / S, Q = S * S / 256;
+
+    static __device__ __forceinline__ int col(int lane) { return lane % S; }
+    static __device__ __forceinline__ int slot(int lane) { return lane / S; }
+    static __device__ __forceinline__ int row4(int q, int lane) { return S == 32 ? 8 * q + 4 * slot(lane) : 4 * slot(lane); }
+
+    static __device__ __forceinline__ Acc mma(const Frag8<T>& a, const Frag8<T>& b, Acc c) {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if constexpr (S == 32) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.e[j], b.e[j], c, 0, 0, 0);
+                else c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.e[j], b.e[j], c, 0, 0, 0);
+            }
+            return c;
+        } else if constexpr (S == 16) {
+            return MfmaOp<T>::run(a.v, b.v, c);
+        } else if constexpr (std::is_same_v<T, f16>) {
+            return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a.v), __builtin_bit_cast(f16x8, b.v), c, 0, 0, 0);
+        } else {
+            return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a.v), __builtin_bit_cast(bf16x8, b.v), c, 0, 0, 0);
+        }
+    }
+    static __device__ __forceinline__ Acc fill(float v) {
+        Acc a;
+#pragma unroll
+        for (int e = 0; e < 4 * Q; ++e) a[e] = v;
+        return a;
+    }
+    static __device__ __forceinline__ f32x4 quad(const Acc& a, int q) { return f32x4{a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]}; }
+
+    // The right operand of product kk (rows kk K .. of a column of tiles) from the
+    // lane's own results
+    static __device__ __forceinline__ Frag8<T> pack(const Acc* tiles, int kk) {
+        typedef T tx8 __attribute__((ext_vector_type(8)));
+        typedef float f32x8 __attribute__((ext_vector_type(8)));
+        f32x8 v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = S == 32 ? tiles[kk / 2][(8 * (kk & 1) + e) % (4 * Q)] : tiles[2 * kk + e / 4][e % 4];
+        return __builtin_bit_cast(Frag8<T>, __builtin_convertvector(v, tx8));
+    }
+
+    // From an LDS tile of rows of W elements: elements ks K + 8 slot .. of row r0 +
+    // lane % S
+    template <int W>
     static __device__ __forceinline__ Frag8<T> frag(const unsigned char* tile, int r0, int ks, int lane) {
-        const int g = lane >> 4, li = lane & 15;
-        const unsigned char* const row = tile + (r0 + li) * kRow;
+        typedef LdsTile<T, W> L;
+        const unsigned char* const row = tile + (r0 + col(lane)) * L::kRow;
+        const int sw = L::swizzle(col(lane));
         if constexpr (sizeof(T) == 2) {
             Frag8<T> f;
-            f.v = *(const u32x4*)(row + (((ks * 4) ^ (g ^ swizzle(li))) << 4));
+            f.v = *(const u32x4*)(row + (((ks * (K / 8)) ^ (slot(lane) ^ sw)) << 4));
             return f;
         } else {
             union {
                 u32x4 q[2];
                 Frag8<T> f;
             } u;
-            const int at = (ks * 8) ^ ((2 * g) ^ swizzle(li));
+            const int at = (ks * (K / 4)) ^ ((2 * slot(lane)) ^ sw);
             u.q[0] = *(const u32x4*)(row + (at << 4));
             u.q[1] = *(const u32x4*)(row + ((at ^ 1) << 4));
             return u.f;
         }
     }
-    // Transposed: column db * 16 + lane % 16 of rows r0 + 4g .. + 3 and r0 + 16
-    // + 4g .. + 3 (g = lane / 16): the left operand that pairs with pack_frag.
-    // For 16-bit types the transposing read: the 16 lanes of a group give the
-    // addresses of 4 rows' 4 chunks of 8 bytes and receive a column each.
+    // Transposed, column db S + lane % S of the K rows from r0 on in the order of
+    // `pack`: rows 4 slot .. + 3 and K / 2 + 4 slot .. + 3. For 16-bit types the
+    // transposing read: the 16 lanes of a group give the addresses of 4 rows'
+    // 4 chunks of 8 bytes and receive a column each.
+    template <int W>
     static __device__ __forceinline__ Frag8<T> frag_t(const unsigned char* tile, int r0, int db, int lane) {
-        const int g = lane >> 4, i = lane & 15;
+        typedef LdsTile<T, W> L;
         Frag8<T> f;
         if constexpr (sizeof(T) == 2) {
             typedef short s16x4 __attribute__((ext_vector_type(4)));
             typedef __attribute__((address_space(3))) s16x4* lds4;
-            const int r = 4 * g + (i >> 2);
-            const unsigned char* const p =
-                tile + (r0 + r) * kRow + (((db * 2) ^ (((i >> 1) & 1) ^ swizzle(r))) << 4) + 8 * (i & 1);
+            const int i = lane & 15, r = 4 * slot(lane) + (i >> 2);
+            const int piece = (S == 32 ? 2 * ((lane >> 4) & 1) : 0) + ((i >> 1) & 1);  // of the S columns
             union {
                 s16x4 h[2];
                 u32x4 v;
             } u;
-            u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)p);
-            u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 16 * kRow));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int rh = r + h * (K / 2);
+                u.h[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (lds4)(tile + (r0 + rh) * L::kRow + (((db * (S / 8)) ^ (piece ^ L::swizzle(rh))) << 4) + 8 * (i & 1)));
+            }
             f.v = u.v;
         } else {
+            const int i = col(lane);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int r = 4 * g + e;
-                const unsigned char* const p = tile + (r0 + r) * kRow + (((db * 4) ^ ((i >> 2) ^ swizzle(r))) << 4) + 4 * (i & 3);
-                f.e[e] = *(const T*)p;
-                f.e[4 + e] = *(const T*)(p + 16 * kRow);
+            for (int e = 0; e < 8; ++e) {
+                const int r = 4 * slot(lane) + e % 4 + e / 4 * (K / 2);
+                f.e[e] = *(const T*)(tile + (r0 + r) * L::kRow + (((db * (S / 4)) ^ ((i >> 2) ^ L::swizzle(r))) << 4) + 4 * (i & 3));
             }
         }
         return f;
     }
-};
 
-__device__ __forceinline__ float across_groups_max(float v) {  // over lanes of equal lane % 16
-    v = fmaxf(v, __shfl_xor(v, 16, 64));
-    return fmaxf(v, __shfl_xor(v, 32, 64));
-}
-__device__ __forceinline__ float across_groups_sum(float v) {
-    v += __shfl_xor(v, 16, 64);
-    return v + __shfl_xor(v, 32, 64);
-}
+    // Over the lanes of one column
+    static __device__ __forceinline__ float col_max(float v) {
+        if constexpr (S == 16) v = fmaxf(v, __shfl_xor(v, 16, 64));
+        return fmaxf(v, __shfl_xor(v, 32, 64));
+    }
+    static __device__ __forceinline__ float col_sum(float v) {
+        if constexpr (S == 16) v += __shfl_xor(v, 16, 64);
+        return v + __shfl_xor(v, 32, 64);
+    }
+};
 
 // Stores 4 consecutive float32 values as T; the row's end may fall inside.
 template <typename T>
@@ -177,28 +218,33 @@ __device__ __forceinline__ Buffer open_buffer(const void* base) {
     return {make_rsrc(base, 0x7fffffffu), u32x4{lo, hi & 0xffffu, 0x7fffffffu, 0x00020000u}};
 }
 
+// Where in LDS a pointer into it points: the low half of its flat address (the
+// high half is the aperture). The same for the wave.
+__device__ __forceinline__ uint32_t lds_offset(const void* p) {
+    return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)p);
+}
+
 // 16 bytes per lane from `offset` in the buffer to 16 lane + `to` in LDS (`to` is
 // the same for the wave). Written as the instruction itself: before any read of
 // LDS the compiler waits for the loads to LDS that it knows of, as it cannot
 // tell which of two tiles they go to, and no load would be in flight during the
-// work on the tile before. There is no output register; `landed` waits.
+// work on the tile before. There is no output register; `landed` waits. m0, which
+// holds the LDS address, is set in the same statement and holds nothing else here.
 __device__ __forceinline__ void load_to_lds(u32x4 r, uint32_t offset, const unsigned char* to) {
-    typedef __attribute__((address_space(3))) const unsigned char* lds;
-    const uint32_t base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds)to);
+    const uint32_t base = lds_offset(to);
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                  :
                  : "s"(base), "v"(offset), "s"(r)
-                 : "memory", "m0");
+                 : "memory");
 }
 
 // The same for 4 bytes per lane.
 __device__ __forceinline__ void load_word_to_lds(u32x4 r, uint32_t offset, const void* to) {
-    typedef __attribute__((address_space(3))) const unsigned char* lds;
-    const uint32_t base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds)to);
+    const uint32_t base = lds_offset(to);
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
                  :
                  : "s"(base), "v"(offset), "s"(r)
-                 : "memory", "m0");
+                 : "memory");
 }
 
 // One thread's share of loading a tile of TILE rows by W elements to LDS through
@@ -273,6 +319,31 @@ struct CrossArgs {
     bool vec;              // D and all strides are multiples of 8 elements, all starts of 16 bytes
 };
 
+__device__ __forceinline__ int64_t seen_length(const CrossArgs& p, int b) {
+    if (!p.lengths) return p.Nk;
+    const int64_t n = p.lengths[b];
+    return n < 0 ? 0 : n > p.Nk ? p.Nk : n;
+}
+
+// Splits are joined by workgroups of 64 chunks of 4 values by 4 thread groups,
+// each of which takes consecutive splits; the groups' sums are added in order.
+constexpr int kJoinGroups = 4;
+__device__ __forceinline__ f32x4 join_groups(f32x4 v, int g, int chunk) {
+    __shared__ f32x4 red[kJoinGroups - 1][64];
+    if (g > 0) red[g - 1][chunk] = v;
+    __syncthreads();
+#pragma unroll
+    for (int q = 1; q < kJoinGroups; ++q) v += red[q - 1][chunk];
+    return v;
+}
+// This thread's share of a chunk's splits, `stride` floats apart, from p on
+__device__ __forceinline__ f32x4 split_sum(const float* p, int64_t stride, int splits, int g) {
+    const int per = (splits + kJoinGroups - 1) / kJoinGroups, s0 = lesser(splits, g * per), n = lesser(splits, s0 + per) - s0;
+    float a[4] = {0.f, 0.f, 0.f, 0.f};
+    add_strided(a, p + s0 * stride, stride, n);
+    return f32x4{a[0], a[1], a[2], a[3]};
+}
+
 // Workgroup -> (sample and key head, tile): the n tiles of a head stay on one
 // XCD, whose L2 then holds its keys (workgroup w runs on XCD w % 8), and
 // neighbouring heads go to different XCDs, so that samples of unequal length
@@ -289,6 +360,22 @@ __device__ __forceinline__ HeadTile head_tile(uint32_t w, uint32_t grid, uint32_
     }
     const uint32_t t = (uint32_t)xcd_tile(w - whole, grid - whole), q = t / n;
     return {(int)(eights * 8 + q), t - q * n};
+}
+
+// The sample whose length has this rank, the longest first: workgroups start in
+// order, and those of long samples must not start last. Up to 64 samples, each
+// lane ranks one (equal lengths by number); others keep their order.
+__device__ __forceinline__ int sample_of_rank(const CrossArgs& p, int rank) {
+    if (!p.lengths || p.B > 64 || p.B == 1) return rank;
+    const int lane = threadIdx.x & 63;
+    const int64_t own = lane < p.B ? seen_length(p, lane) : -1;
+    const int n = (int)lesser<int64_t>(own, 0x7fffffff);
+    int r = 0;
+    for (int b = 0; b < p.B; ++b) {
+        const int other = __builtin_amdgcn_readlane(n, b);
+        r += other > n || (other == n && b < lane);
+    }
+    return __builtin_ctzll(__ballot(lane < p.B && r == rank));
 }
 
 // Row r of the M rows of key head `j`: the offset of its query and head
@@ -313,12 +400,6 @@ __device__ __forceinline__ uint32_t row_tile_at(const CrossArgs& p, const RowTil
     if (p.G == 1) return (uint32_t)(i * (int)sn) * size;
     const int x = i + t.rem, n = (int)((x + 0.5f) * p.inv_g);  // x below 2^20: exact
     return (uint32_t)(n * (int)sn + (x - n * p.G) * (int)sh) * size;
-}
-
-__device__ __forceinline__ int64_t seen_length(const CrossArgs& p, int b) {
-    if (!p.lengths) return p.Nk;
-    const int64_t n = p.lengths[b];
-    return n < 0 ? 0 : n > p.Nk ? p.Nk : n;
 }
 
 }  // namespace svtad

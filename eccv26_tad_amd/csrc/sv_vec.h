@@ -33,4 +33,18 @@ __device__ __forceinline__ float group_sum(float v, int lanes) {
     return v;
 }
 
+// Sum of count float4 at p, p + stride, ... (floats), in order, four loads in
+// flight
+__device__ __forceinline__ void add_strided(float (&acc)[4], const float* p, int64_t stride, int count) {
+    for (int i = 0; i < count; i += 4) {
+        Pack<float, 4> v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = *(const Pack<float, 4>*)(p + (i + u < count ? i + u : count - 1) * stride);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] += i + u < count ? v[u].e[e] : 0.f;
+    }
+}
+
 }  // namespace svtad

@@ -7,31 +7,8 @@ the query and key rows of the adapter's heads (``:598-606``).
 from __future__ import annotations
 
 import torch
-from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import opentad_sparse_ops as _ops
-
-
-class LayerNormFunction(Function):
-    """autograd node of ``layer_norm``; keeps x and each row's mean and
-    reciprocal deviation for the backward."""
-
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        y, stats = _ops.layer_norm(x, weight, bias, eps, True)
-        ctx.save_for_backward(x, stats, weight)
-        given = weight if weight is not None else bias
-        ctx.params_f32 = given is not None and given.dtype == torch.float32
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, stats, weight = ctx.saved_tensors
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dx, dw, db = _ops.layer_norm_bwd(dy, x, stats, weight, ctx.params_f32, need_x, need_w, need_b)
-        return dx, dw, db, None
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
@@ -49,5 +26,5 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
         weight, bias = (None if p is None else p.float() for p in (weight, bias))
         given = [p for p in (weight, bias) if p is not None]
     if torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in given)):
-        return LayerNormFunction.apply(x, weight, bias, eps)
+        return _ops.layer_norm_grad(x, weight, bias, eps)
     return _ops.layer_norm(x, weight, bias, eps, False)[0]

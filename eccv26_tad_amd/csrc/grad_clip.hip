@@ -16,6 +16,7 @@
 // bytes). Every workgroup leaves one partial sum; the scaling pass adds them
 // in one fixed order in each of its workgroups, without a launch between.
 #include <algorithm>
+#include <type_traits>
 
 #include "sv_internal.h"
 #include "sv_vec.h"
@@ -42,16 +43,29 @@ struct ClipScale {
     bool inf;
 };
 
-// First tensor whose end is past element e
-__device__ __forceinline__ int clip_find(const ClipList& t, int64_t e) {
-    int lo = 0, hi = t.count - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (t.end[mid] > e) hi = mid;
-        else lo = mid + 1;
+// The list in LDS, one entry per thread: kernel arguments lie in host memory, and
+// a search through them there waits for one far load after another (81 M elements
+// of 160 tensors in bfloat16: 52 us against 50).
+struct ClipTable {
+    const void* g[kTensors];
+    void* out[kTensors];
+    int64_t end[kTensors];
+    int first[4];
+
+    // Fills it; the first tensor whose end is past element e
+    __device__ __forceinline__ int open(const ClipList& t, int64_t e) {
+        const int i = threadIdx.x;
+        bool past = false;
+        if (i < t.count) {
+            g[i] = t.g[i], out[i] = t.out[i], end[i] = t.end[i];
+            past = t.end[i] > e;
+        }
+        const uint64_t m = __ballot(i < t.count && !past);
+        if ((i & 63) == 0) first[i >> 6] = __popcll(m);
+        __syncthreads();
+        return first[0] + first[1] + first[2] + first[3];
     }
-    return lo;
-}
+};
 
 template <bool INF>
 __device__ __forceinline__ double clip_join(double a, double b) {
@@ -70,7 +84,22 @@ __device__ __forceinline__ double clip_reduce(double v) {
     return clip_join<INF>(clip_join<INF>(red[0], red[1]), clip_join<INF>(red[2], red[3]));
 }
 
-constexpr int kUnroll = 4;  // 16-byte loads in flight per thread
+// n elements of a workgroup, V at a time: vectors(offset, count) for count vectors,
+// 256 V elements apart, from where `lines` (elements of S bytes, the wider of what
+// is read and written) reaches a cache line on, one(offset) for the others. A
+// tensor inside a bucket starts anywhere; a wave that stores parts of lines alone
+// costs a third more.
+template <int S, int V, int UNROLL, typename F, typename G>
+__device__ __forceinline__ void clip_walk(const void* lines, int64_t n, F vectors, G one) {
+    int64_t head = ((128 - ((uintptr_t)lines & 127)) & 127) / S;
+    head = head < n ? head : n;
+    const int64_t end = head + (n - head) / V * V;
+    if ((int64_t)threadIdx.x < head) one((int64_t)threadIdx.x);
+    int64_t at = head + threadIdx.x * V;
+    for (; at + (UNROLL - 1) * 256 * V < end; at += UNROLL * 256 * V) vectors(at, std::integral_constant<int, UNROLL>());
+    for (; at < end; at += 256 * V) vectors(at, std::integral_constant<int, 1>());
+    if (end + threadIdx.x < n) one(end + threadIdx.x);
+}
 
 template <typename T, bool INF>
 __global__ __launch_bounds__(256) void k_grad_norm(ClipList t, double* part) {
@@ -79,35 +108,30 @@ __global__ __launch_bounds__(256) void k_grad_norm(ClipList t, double* part) {
     const int64_t per = cdiv(cdiv(total, gridDim.x), 64) * 64;
     int64_t e = (int64_t)blockIdx.x * per;
     const int64_t e1 = min<int64_t>(total, e + per);
-    double acc = 0.0;
-    auto add = [&](T v) {
+    double acc[4] = {0.0, 0.0, 0.0, 0.0};
+    auto add = [&](T v, int k) {
         const double d = (double)(float)v;
-        acc = INF ? clip_join<true>(acc, fabs(d)) : fma(d, d, acc);
+        acc[k] = INF ? clip_join<true>(acc[k], fabs(d)) : fma(d, d, acc[k]);
     };
-    for (int i = e < e1 ? clip_find(t, e) : 0; e < e1; ++i) {
-        const int64_t first = i ? t.end[i - 1] : 0, stop = min<int64_t>(e1, t.end[i]);
-        const T* const g = (const T*)t.g[i] + (e - first);
-        const int64_t n = stop - e, body = n / (256 * V) * (256 * V);
-        int64_t at = threadIdx.x * V;
-        for (; at + (kUnroll - 1) * 256 * V < body; at += kUnroll * 256 * V) {
-            Pack<T, V> v[kUnroll];
+    __shared__ ClipTable tab;
+    for (int i = tab.open(t, e); e < e1; ++i) {
+        const int64_t first = i ? tab.end[i - 1] : 0, stop = min<int64_t>(e1, tab.end[i]);
+        const T* const g = (const T*)tab.g[i] + (e - first);
+        clip_walk<(int)sizeof(T), V, 4>(g, stop - e,
+            [&](int64_t at, auto unroll) {
+                Pack<T, V> v[unroll.value];
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u) v[u] = *(const Pack<T, V>*)(g + at + u * 256 * V);
+                for (int u = 0; u < unroll.value; ++u) v[u] = load_once<Pack<T, V>>(g + at + u * 256 * V);
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u)
+                for (int u = 0; u < unroll.value; ++u)
 #pragma unroll
-                for (int k = 0; k < V; ++k) add(v[u].e[k]);
-        }
-        for (; at < body; at += 256 * V) {
-            const Pack<T, V> v = *(const Pack<T, V>*)(g + at);
-#pragma unroll
-            for (int k = 0; k < V; ++k) add(v.e[k]);
-        }
-        for (int64_t q = body + threadIdx.x; q < n; q += 256) add(g[q]);
+                    for (int k = 0; k < V; ++k) add(v[u].e[k], k & 3);
+            },
+            [&](int64_t at) { add(g[at], 0); });
         e = stop;
     }
-    acc = clip_reduce<INF>(acc);
-    if (threadIdx.x == 0) part[blockIdx.x] = acc;
+    const double sum = clip_reduce<INF>(clip_join<INF>(clip_join<INF>(acc[0], acc[1]), clip_join<INF>(acc[2], acc[3])));
+    if (threadIdx.x == 0) part[blockIdx.x] = sum;
 }
 
 // The norm of all partial sums (before scale), in every thread
@@ -130,7 +154,10 @@ __global__ __launch_bounds__(256) void k_grad_norm_out(ClipScale s) {
 // still.
 template <typename T, typename O>
 __global__ __launch_bounds__(256) void k_grad_scale(ClipList t, ClipScale s) {
-    constexpr int V = kVec<T>;
+    // as many elements as the wider of the two types has in 16 bytes, so that a
+    // wave's stores are whole lines (twice 16 bytes per lane: 207 us against 150)
+    constexpr int V = 16 / (sizeof(T) > sizeof(O) ? (int)sizeof(T) : (int)sizeof(O));
+    constexpr int kBytesInFlight = 64;  // of loads, per thread
     const double n = clip_norm(s) * fabs((double)s.scale);
     if (s.norm && blockIdx.x == 0 && threadIdx.x == 0) *s.norm = (float)n;
     double c = s.limit < 0.f ? 1.0 : (double)s.limit / (n + kClipEps);
@@ -142,40 +169,34 @@ __global__ __launch_bounds__(256) void k_grad_scale(ClipList t, ClipScale s) {
     const int64_t per = cdiv(cdiv(total, gridDim.x), 64) * 64;
     int64_t e = (int64_t)(gridDim.x - 1 - blockIdx.x) * per;
     const int64_t e1 = min<int64_t>(total, e + per);
-    for (int i = e < e1 ? clip_find(t, e) : 0; e < e1; ++i) {
-        const int64_t first = i ? t.end[i - 1] : 0, stop = min<int64_t>(e1, t.end[i]);
-        const T* const g = (const T*)t.g[i] + (e - first);
-        O* const o = (O*)t.out[i] + (e - first);
-        const int64_t m = stop - e, body = m / (256 * V) * (256 * V);
-        int64_t at = threadIdx.x * V;
-        for (; at + (kUnroll - 1) * 256 * V < body; at += kUnroll * 256 * V) {
-            Pack<T, V> v[kUnroll];
+    __shared__ ClipTable tab;
+    for (int i = tab.open(t, e); e < e1; ++i) {
+        const int64_t first = i ? tab.end[i - 1] : 0, stop = min<int64_t>(e1, tab.end[i]);
+        const T* const g = (const T*)tab.g[i] + (e - first);
+        O* const o = (O*)tab.out[i] + (e - first);
+        clip_walk<16 / V, V, kBytesInFlight / (V * (int)sizeof(T))>(
+            sizeof(T) > sizeof(O) ? (const void*)g : o, stop - e,
+            [&](int64_t at, auto unroll) {
+                Pack<T, V> v[unroll.value];
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u) v[u] = *(const Pack<T, V>*)(g + at + u * 256 * V);
+                for (int u = 0; u < unroll.value; ++u) v[u] = load_once<Pack<T, V>>(g + at + u * 256 * V);
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u) {
-                Pack<O, V> w;
+                for (int u = 0; u < unroll.value; ++u) {
+                    Pack<O, V> w;
 #pragma unroll
-                for (int k = 0; k < V; ++k) w.e[k] = (O)((float)v[u].e[k] * f);
-                *(Pack<O, V>*)(o + at + u * 256 * V) = w;
-            }
-        }
-        for (; at < body; at += 256 * V) {
-            const Pack<T, V> v = *(const Pack<T, V>*)(g + at);
-            Pack<O, V> w;
-#pragma unroll
-            for (int k = 0; k < V; ++k) w.e[k] = (O)((float)v.e[k] * f);
-            *(Pack<O, V>*)(o + at) = w;
-        }
-        for (int64_t q = body + threadIdx.x; q < m; q += 256) o[q] = (O)((float)g[q] * f);
+                    for (int k = 0; k < V; ++k) w.e[k] = (O)((float)v[u].e[k] * f);
+                    store_once(o + at + u * 256 * V, w);
+                }
+            },
+            [&](int64_t at) { o[at] = (O)((float)g[at] * f); });
         e = stop;
     }
 }
 
 // Workgroups for `total` elements: one for every 16 KB or so, at most four per
-// compute unit.
-static int clip_groups(int64_t total) {
-    return (int)std::max<int64_t>(1, std::min<int64_t>(cdiv(total, 4096), kMaxGroups));
+// compute unit in the norm's pass (each leaves a partial sum), eight in the other.
+static int clip_groups(int64_t total, int most = kMaxGroups) {
+    return (int)std::max<int64_t>(1, std::min<int64_t>(cdiv(total, 4096), most));
 }
 
 struct ClipPlan {  // the launches of a list of tensors of any length
@@ -245,7 +266,7 @@ extern "C" size_t svtad_grad_clip_workspace_bytes(const svtad_grad* tensors, int
 }
 
 extern "C" int svtad_grad_clip(const svtad_grad* tensors, int64_t count, int norm_type, float max_norm, float scale,
-                               int write, float* norm, void* workspace, size_t workspace_bytes, void* stream) {
+                         int write, float* norm, void* workspace, size_t workspace_bytes, void* stream) {
     const int st = clip_check(tensors, count, write != 0);
     if (st) return st;
     if (norm_type != SVTAD_NORM_2 && norm_type != SVTAD_NORM_INF)
@@ -260,8 +281,10 @@ extern "C" int svtad_grad_clip(const svtad_grad* tensors, int64_t count, int nor
     double* const part = (double*)workspace;
     const bool inf = norm_type == SVTAD_NORM_INF;
     ClipList l;
-    int64_t done = 0;
+    int64_t done = 0, starts[64];  // where launches begin; the 64th stands for all that follow
+    int n_starts = 0;
     for (int64_t at = 0; at < count;) {
+        if (n_starts < 64) starts[n_starts++] = at;
         at = plan.take(at, l);
         if (!l.count) continue;
         const int grid = clip_groups(l.end[l.count - 1]);
@@ -275,14 +298,19 @@ extern "C" int svtad_grad_clip(const svtad_grad* tensors, int64_t count, int nor
         k_grad_norm_out<<<1, 256, 0, hs>>>(s);
         return launch_status();
     }
-    for (int64_t at = 0; at < count;) {
-        at = plan.take(at, l);
-        if (!l.count) continue;
-        const int grid = clip_groups(l.end[l.count - 1]);
-        if (l.g_type == SVTAD_F32) launch_scale<float>(l, s, grid, hs);
-        else if (l.g_type == SVTAD_F16) launch_scale<f16>(l, s, grid, hs);
-        else launch_scale<bf16>(l, s, grid, hs);
-        s.norm = nullptr;
+    // the last launch's tensors first: the cache holds them still
+    for (int i = n_starts - 1; i >= 0; --i) {
+        int64_t at = starts[i];
+        const int64_t stop = i + 1 < n_starts ? starts[i + 1] : count;
+        while (at < stop) {
+            at = plan.take(at, l);
+            if (!l.count) continue;
+            const int grid = clip_groups(l.end[l.count - 1], 2 * kMaxGroups);
+            if (l.g_type == SVTAD_F32) launch_scale<float>(l, s, grid, hs);
+            else if (l.g_type == SVTAD_F16) launch_scale<f16>(l, s, grid, hs);
+            else launch_scale<bf16>(l, s, grid, hs);
+            s.norm = nullptr;
+        }
     }
     return launch_status();
 }

@@ -152,7 +152,39 @@ __global__ __launch_bounds__(256) void k_layer_norm(LnArgs p) {
     }
 }
 
-// dx, and the workgroup's partial sums of dy xhat and dy in p.part
+// A row's vectors of x and dy as they lie in memory, and its statistics
+template <typename T, int K, bool TAIL>
+struct LnRow {
+    static constexpr int V = kVec<T>;
+    Pack<T, V> x[K], d[K];
+    float mean, rstd;
+    bool in;
+
+    __device__ __forceinline__ void load(const LnArgs& p, int64_t r, int G, int g) {
+        in = r < p.rows;
+        const T* const x0 = (const T*)p.x + (in ? row_offset(r, p.n1, p.n2, p.s0, p.s1, p.s2) : 0);
+        const T* const d0 = (const T*)p.dy + (in ? row_offset(r, p.n1, p.n2, p.t0, p.t1, p.t2) : 0);
+        const int c = in ? p.c : 0;
+        mean = in ? p.stats[r * 2] : 0.f, rstd = in ? p.stats[r * 2 + 1] : 0.f;
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+            const int c0 = (j * G + g) * V;
+            if (c0 + V <= c) {
+                x[j] = *(const Pack<T, V>*)(x0 + c0);
+                d[j] = *(const Pack<T, V>*)(d0 + c0);
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    x[j].e[e] = TAIL && c0 + e < c ? x0[c0 + e] : (T)0.f;
+                    d[j].e[e] = TAIL && c0 + e < c ? d0[c0 + e] : (T)0.f;  // 0 past the row's end, as the sums need it
+                }
+            }
+        }
+    }
+};
+
+// dx, and the workgroup's partial sums of dy xhat and dy in p.part. The next
+// row's loads are in flight while a row's sums are exchanged.
 template <typename T, int K, bool WG, bool TAIL>
 __global__ __launch_bounds__(256) void k_layer_norm_bwd(LnArgs p) {
     constexpr int V = kVec<T>, W = 64 * K * V;  // the widest row of a wave's group
@@ -166,21 +198,20 @@ __global__ __launch_bounds__(256) void k_layer_norm_bwd(LnArgs p) {
         for (int e = 0; e < V; ++e) sw[j][e] = sb[j][e] = 0.f;
     }
     const float ic = 1.f / c;
-    for (int64_t r0 = (int64_t)blockIdx.x * per; r0 < p.rows; r0 += (int64_t)gridDim.x * per) {
+    const int64_t step = (int64_t)gridDim.x * per;
+    LnRow<T, K, TAIL> next;
+    next.load(p, (int64_t)blockIdx.x * per + threadIdx.x / G, G, g);
+    for (int64_t r0 = (int64_t)blockIdx.x * per; r0 < p.rows; r0 += step) {
         const int64_t r = r0 + threadIdx.x / G;
-        const bool in = r < p.rows;
-        const T* const x = (const T*)p.x + (in ? row_offset(r, p.n1, p.n2, p.s0, p.s1, p.s2) : 0);
-        const T* const dy = (const T*)p.dy + (in ? row_offset(r, p.n1, p.n2, p.t0, p.t1, p.t2) : 0);
-        const float mean = in ? p.stats[r * 2] : 0.f, rstd = in ? p.stats[r * 2 + 1] : 0.f;
+        const LnRow<T, K, TAIL> row = next;
+        if (r0 + step < p.rows) next.load(p, r + step, G, g);
         float xh[K][V], d[K][V], s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int j = 0; j < K; ++j) {
-            load_vec<T, TAIL>(xh[j], x, in ? (j * G + g) * V : c, c);
-            load_vec<T, TAIL>(d[j], dy, in ? (j * G + g) * V : c, c);  // 0 past the row's end, as the sums need it
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                xh[j][e] = (xh[j][e] - mean) * rstd;
-                const float t = d[j][e];
+                xh[j][e] = ((float)row.x[j].e[e] - row.mean) * row.rstd;
+                const float t = (float)row.d[j].e[e];
                 sw[j][e] += t * xh[j][e];
                 sb[j][e] += t;
                 d[j][e] = t * w[j][e];
@@ -191,12 +222,12 @@ __global__ __launch_bounds__(256) void k_layer_norm_bwd(LnArgs p) {
         if (!p.y) continue;
         s1 = row_sum<WG>(s1, min(G, 64), red) * ic;
         s2 = row_sum<WG>(s2, min(G, 64), red) * ic;
-        if (!in) continue;
+        if (!row.in) continue;
         T* const dx = (T*)p.y + r * c;
 #pragma unroll
         for (int j = 0; j < K; ++j) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) d[j][e] = rstd * (d[j][e] - s1 - xh[j][e] * s2);
+            for (int e = 0; e < V; ++e) d[j][e] = row.rstd * (d[j][e] - s1 - xh[j][e] * s2);
             store_vec<T, TAIL>(dx, d[j], (j * G + g) * V, c);
         }
     }

@@ -13,6 +13,29 @@ struct __attribute__((packed, aligned(sizeof(T)))) Pack {
     T e[N];
 };
 
+// 8 or 16 bytes of global memory that are read, or written, once: they are not
+// kept in the caches (1 GiB read through: 7.0 against 6.1 TB/s; copied: 5.6
+// against 5.3). A wave's stores should fill whole lines: nothing merges them. The
+// address space is given because pointers that were kept in LDS do not tell.
+template <int BYTES> struct OnceType;
+template <> struct OnceType<16> {
+    typedef unsigned int type __attribute__((ext_vector_type(4), aligned(2)));
+};
+template <> struct OnceType<8> {
+    typedef unsigned int type __attribute__((ext_vector_type(2), aligned(2)));
+};
+template <typename P>
+__device__ __forceinline__ P load_once(const void* p) {
+    typedef __attribute__((address_space(1))) const typename OnceType<sizeof(P)>::type* global;
+    return __builtin_bit_cast(P, __builtin_nontemporal_load((global)p));
+}
+template <typename P>
+__device__ __forceinline__ void store_once(void* p, const P& v) {
+    typedef typename OnceType<sizeof(P)>::type U;
+    typedef __attribute__((address_space(1))) U* global;
+    __builtin_nontemporal_store(__builtin_bit_cast(U, v), (global)p);
+}
+
 // Elements of 16 bytes.
 template <typename T> constexpr int kVec = 16 / (int)sizeof(T);
 

@@ -260,37 +260,52 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> op_cross_attention_bwd(
     return {dq, dk, dv};
 }
 
-// grad_clip(grads, outs (empty: the norm alone), max_norm (negative: no limit), scale, inf) -> norm, a float32 scalar
-at::Tensor op_grad_clip(const std::vector<at::Tensor>& grads, const std::vector<at::Tensor>& outs, double max_norm,
-                        double scale, bool inf) {
+// grad_clip(grads, outs (None: in place), write, max_norm (negative: no limit), scale, inf) -> norm, a float32
+// scalar; without write the norm alone. Tensors whose elements do not fill one span of memory go by way of a copy.
+at::Tensor op_grad_clip(const std::vector<at::Tensor>& grads, const c10::optional<std::vector<at::Tensor>>& outs, bool write,
+                        double max_norm, double scale, bool inf) {
     TORCH_CHECK(!grads.empty(), "opentad_sparse_ops.grad_clip: no tensors");
-    const bool write = !outs.empty();
-    TORCH_CHECK(!write || outs.size() == grads.size(), "opentad_sparse_ops.grad_clip: ", grads.size(), " gradients and ",
-                outs.size(), " outputs");
+    const bool apart = write && outs.has_value();
+    TORCH_CHECK(!apart || outs->size() == grads.size(), "opentad_sparse_ops.grad_clip: ", grads.size(), " gradients and ",
+                apart ? outs->size() : 0, " outputs");
+    at::NoGradGuard no_grad;
+    c10::DeviceGuard g(grads[0].device());
     std::vector<svtad_grad> list(grads.size());
+    std::vector<at::Tensor> copies;
+    std::vector<size_t> copied;
     for (size_t i = 0; i < grads.size(); ++i) {
-        const at::Tensor& t = grads[i];
+        at::Tensor t = grads[i];
         check_float(t, "gradients");
         TORCH_CHECK(t.device() == grads[0].device(), "opentad_sparse_ops.grad_clip: gradients must be on one device");
-        TORCH_CHECK(t.is_non_overlapping_and_dense(), "opentad_sparse_ops.grad_clip: gradients must be dense");
+        if (!t.is_non_overlapping_and_dense()) {
+            t = t.contiguous();
+            copies.push_back(t);
+            if (!apart) copied.push_back(i);
+        }
         list[i].g = t.data_ptr(), list[i].count = t.numel(), list[i].g_type = dtype_code(t);
         if (!write) continue;
-        const at::Tensor& o = outs[i];
-        check_float(o, "outputs");
-        TORCH_CHECK(o.device() == t.device() && o.sizes() == t.sizes() &&
-                        ((o.is_contiguous() && t.is_contiguous()) || o.strides() == t.strides()),
-                    "opentad_sparse_ops.grad_clip: an output must have its gradient's device, shape and strides");
-        TORCH_CHECK(t.numel() == 0 || o.data_ptr() != t.data_ptr() || o.scalar_type() == t.scalar_type(),
-                    "opentad_sparse_ops.grad_clip: in place an output must have its gradient's dtype");
+        const at::Tensor& o = apart ? (*outs)[i] : t;
+        if (apart) {
+            check_float(o, "outputs");
+            TORCH_CHECK(o.device() == t.device() && o.sizes() == t.sizes() &&
+                            ((o.is_contiguous() && t.is_contiguous()) || o.strides() == t.strides()),
+                        "opentad_sparse_ops.grad_clip: an output must have its gradient's device, shape and strides");
+            TORCH_CHECK(t.numel() == 0 || o.data_ptr() != t.data_ptr() || o.scalar_type() == t.scalar_type(),
+                        "opentad_sparse_ops.grad_clip: in place an output must have its gradient's dtype");
+        }
         list[i].out = o.data_ptr(), list[i].out_type = dtype_code(o);
+        if (!o.is_inference()) o.unsafeGetTensorImpl()->bump_version();
     }
-    c10::DeviceGuard g(grads[0].device());
     at::Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
     const size_t bytes = svtad_grad_clip_workspace_bytes(list.data(), (int64_t)list.size());
     at::Tensor ws = workspace(bytes, grads[0]);
     check_status(svtad_grad_clip(list.data(), (int64_t)list.size(), inf ? SVTAD_NORM_INF : SVTAD_NORM_2, (float)max_norm,
                                  (float)scale, write, norm.data_ptr<float>(), ptr(ws), bytes, stream_of(grads[0])),
                  "grad_clip");
+    if (write) {
+        size_t at = 0;
+        for (size_t i : copied) grads[i].copy_(copies[at++]);
+    }
     return norm;
 }
 
@@ -410,5 +425,5 @@ void bind_operators(pybind11::module& m) {
           py::arg("k"), py::arg("v"), py::arg("out"), py::arg("lse"), py::arg("key_lengths"), py::arg("key_mask"),
           py::arg("scale"), py::arg("need_q"), py::arg("need_kv"));
     m.def("grad_clip", &op_grad_clip, "The norm over all gradients, and the gradients scaled down to a limit",
-          py::arg("grads"), py::arg("outs"), py::arg("max_norm"), py::arg("scale"), py::arg("inf"));
+          py::arg("grads"), py::arg("outs"), py::arg("write"), py::arg("max_norm"), py::arg("scale"), py::arg("inf"));
 }

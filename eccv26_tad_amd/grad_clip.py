@@ -21,18 +21,12 @@ def _is_inf(norm_type) -> bool:
     return norm_type == math.inf
 
 
-def _dense(t):
-    """Whether the elements of ``t`` fill one span of memory, each once."""
-    return t.is_contiguous() or torch.ops.aten.is_non_overlapping_and_dense(t)
-
-
 def grad_norm(grads: Sequence[torch.Tensor], norm_type: float = 2.0, scale: float = 1.0) -> torch.Tensor:
     """``|scale|`` times the 2-norm (or, for ``inf``, the largest magnitude) of
     all elements of ``grads``: a float32 scalar on the GPU."""
-    return _ops.grad_clip([g if _dense(g) else g.contiguous() for g in grads], [], -1.0, scale, _is_inf(norm_type))
+    return _ops.grad_clip(grads, None, False, -1.0, scale, _is_inf(norm_type))
 
 
-@torch.no_grad()
 def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float = 2.0,
                out: Sequence[torch.Tensor] | None = None, scale: float = 1.0) -> torch.Tensor:
     """Scale ``grads`` by ``scale`` and down to a norm of ``max_norm``: each
@@ -47,15 +41,7 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float 
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError(f"clip_grads: max_norm must not be negative, got {max_norm}")
-    inf = _is_inf(norm_type)
-    if out is None and not all(_dense(g) for g in grads):
-        copies = [g if _dense(g) else g.contiguous() for g in grads]
-        norm = _ops.grad_clip(copies, copies, max_norm, scale, inf)
-        for g, c in zip(grads, copies):
-            if c is not g:
-                g.copy_(c)
-        return norm
-    return _ops.grad_clip(grads, grads if out is None else out, max_norm, scale, inf)
+    return _ops.grad_clip(grads, out, True, max_norm, scale, _is_inf(norm_type))
 
 
 def clip_grad_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm: float, norm_type: float = 2.0,

@@ -13,7 +13,7 @@ template <typename T> void cross_bwd_kv(const CrossArgs& p, hipStream_t st);
 
 // Workgroups of 4 waves that a compute unit is to hold, by what a kernel keeps in
 // registers. At 64 channels (ViT-L training case, two / three of them): forward
-// 615 / 553 us, dq 650 / 658, dk and dv 798 / 913 (three spill).
+// 570 / 538 us, dq 650 / 658, dk and dv 798 / 913 (three spill).
 template <typename T, int DP> constexpr int kResidentFwd = sizeof(T) == 2 && DP <= 64 ? 3 : 1;
 template <typename T, int DP> constexpr int kResidentBwd = sizeof(T) == 2 && DP <= 64 ? 2 : 1;
 

@@ -86,7 +86,7 @@ static bool whole_vectors(const svtad_cross_args& a, const void* p, const int64_
            (heads <= 1 || s[2] % 8 == 0);
 }
 
-static CrossArgs cross_args(const svtad_cross_args& a) {
+static CrossArgs cross_args(const svtad_cross_args& a, int dtype) {
     CrossArgs p{};
     p.q = a.q, p.k = a.k, p.v = a.v;
     p.qb = a.q_stride[0], p.qn = a.q_stride[1], p.qh = a.q_stride[2];
@@ -101,6 +101,9 @@ static CrossArgs cross_args(const svtad_cross_args& a) {
     p.inv_g = 1.f / p.G;
     p.vec = a.head_dim % 8 == 0 && whole_vectors(a, a.q, a.q_stride, a.nq, a.heads) &&
             whole_vectors(a, a.k, a.k_stride, a.nk, a.kv_heads) && whole_vectors(a, a.v, a.v_stride, a.nk, a.kv_heads);
+    p.up = p.down = 1.f;
+    if (dtype == SVTAD_F16)
+        for (int64_t n = 2; n <= a.nk && n <= 8192; n *= 2) p.up *= 2.f, p.down *= 0.5f;
     p.splits = 1;
     return p;
 }
@@ -127,7 +130,7 @@ extern "C" int svtad_cross_attention(const svtad_cross_args* a, void* out, float
     if (need && (!workspace || workspace_bytes < need))
         return set_error(SVTAD_ERR_WORKSPACE, "cross_attention: workspace too small");
     const RowPlan plan = row_plan(*a);
-    CrossArgs p = cross_args(*a);
+    CrossArgs p = cross_args(*a, dtype);
     p.out = out, p.lse = lse;
     p.splits = plan.splits, p.part = (float*)workspace;
     if (dtype == SVTAD_F16) cross_fwd<f16>(p, plan.wave_rows, (hipStream_t)stream);
@@ -162,7 +165,7 @@ extern "C" int svtad_cross_attention_bwd(const svtad_cross_args* a, const void* 
     const size_t need = bwd_bytes(*a);
     if (need && (!workspace || workspace_bytes < need))
         return set_error(SVTAD_ERR_WORKSPACE, "cross_attention_bwd: workspace too small");
-    CrossArgs p = cross_args(*a);
+    CrossArgs p = cross_args(*a, dtype);
     p.o = out, p.on = (int64_t)a->heads * a->head_dim, p.oh = a->head_dim, p.ob = a->nq * p.on;
     p.dout = dout;
     if (dout_stride && !near_strides(dout_stride, p.G, dtype))

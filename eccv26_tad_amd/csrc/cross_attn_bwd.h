@@ -10,7 +10,9 @@
 // and dv; the rows of a key head are those of all its query heads). Both
 // recompute the scores, which costs two of the seven products and saves the
 // score matrix in memory. p and ds are rounded to T as operands of the second
-// products; all sums are float32.
+// products; all sums are float32. A probability among n keys is near 1 / n, which
+// float16 holds with few bits (below 2^-14 fewer with every halving): for dv they
+// are scaled up by a power of two, at most n, and the sum down again.
 #pragma once
 
 #include "cross_attn_fwd.h"
@@ -26,7 +28,7 @@ __global__ __launch_bounds__(256, (kResidentBwd<T, DP>)) void k_cross_bwd_q(Cros
     typedef KeyTiles<T, TK, W, VEC> Keys;
     constexpr size_t kJoin = WK > 1 ? (size_t)WK * ROWS * DB * S * 4 : 0;
     __shared__ __attribute__((aligned(16))) unsigned char mem[Keys::kBytes > kJoin ? Keys::kBytes : kJoin];
-    __shared__ __attribute__((aligned(16))) uint8_t seen_mem[Keys::kBuffers * TK];
+    __shared__ __attribute__((aligned(16))) float start_mem[Keys::kBuffers * TK];
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave % WM, wk = wave / WM;
     const int li = M::col(lane), slot = M::slot(lane);
@@ -61,31 +63,22 @@ __global__ __launch_bounds__(256, (kResidentBwd<T, DP>)) void k_cross_bwd_q(Cros
     Acc acc[DB];
 #pragma unroll
     for (int db = 0; db < DB; ++db) acc[db] = M::fill(0.f);
-    Keys keys(p, b, j, split, mem, seen_mem);
+    Keys keys(p, b, j, split, mem, start_mem);
     auto use = [&](int64_t tile, auto part) __attribute__((always_inline)) {
         const unsigned char *const lk = keys.keys(tile), *const lv = keys.values(tile);
-        const int left = keys.left(tile);
 #pragma unroll
         for (int n0 = 0; n0 < KW; n0 += NP * S) {  // NP score tiles make whole products
             Acc ds[NP];
 #pragma unroll
             for (int h = 0; h < NP; ++h) {
                 const int row = wk * KW + n0 + h * S;
-                Acc s = M::fill(0.f), dp = M::fill(-delta);  // the product's own sum: dp - delta
+                Acc s, dp = M::fill(-delta);  // the product's own sum: dp - delta
+                if constexpr (part.value) s = start_scores<M>(keys.start(tile) + row, lane);
+                else s = M::fill(0.f);
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) s = M::mma(M::template frag<W>(lk, row, ks, lane), qf[ks], s);
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) dp = M::mma(M::template frag<W>(lv, row, ks, lane), df[ks], dp);
-                if constexpr (part.value) {  // an unseen key was staged as zeros: its score is 0, not -inf
-#pragma unroll
-                    for (int q = 0; q < M::Q; ++q) {
-                        const int at = row + M::row4(q, lane);
-                        const uint32_t w = keys.mask ? *(const uint32_t*)(keys.seen(tile) + at) : 0x01010101u;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            s[4 * q + e] = at + e < left && ((w >> (8 * e)) & 0xff) ? s[4 * q + e] : kNegInf;
-                    }
-                }
 #pragma unroll
                 for (int e = 0; e < 4 * M::Q; ++e) ds[h][e] = __builtin_amdgcn_exp2f(fmaf(s[e], p.c, -lse)) * dp[e];
             }
@@ -241,6 +234,7 @@ __global__ __launch_bounds__(256, (kResidentBwd<T, DP>)) void k_cross_bwd_kv(Cro
                 for (int e = 0; e < 4; ++e) {
                     s[4 * q + e] = __builtin_amdgcn_exp2f(fmaf(s[4 * q + e], p.c, -l4[e]));
                     dp[4 * q + e] *= s[4 * q + e];
+                    if constexpr (std::is_same_v<T, f16>) s[4 * q + e] *= p.up;
                 }
             }
 #pragma unroll
@@ -270,7 +264,7 @@ __global__ __launch_bounds__(256, (kResidentBwd<T, DP>)) void k_cross_bwd_kv(Cro
 #pragma unroll
         for (int q = 0; q < M::Q; ++q) {
             const int c = db * S + M::row4(q, lane);
-            const f32x4 gk = seen ? M::quad(dk[db], q) : zero, gv = seen ? M::quad(dv[db], q) : zero;
+            const f32x4 gk = seen ? M::quad(dk[db], q) : zero, gv = seen ? M::quad(dv[db], q) * p.down : zero;
             if (p.splits == 1) {
                 store4<T>((T*)p.dk + at, c, p.D, gk * p.scale);
                 store4<T>((T*)p.dv + at, c, p.D, gv);

@@ -23,19 +23,22 @@ namespace svtad {
 constexpr float kNegInf = -__builtin_huge_valf();
 
 // A row's powers are taken relative to the largest score seen when its scale was
-// last set. The scale is set again only when a lane's powers of one tile add up
-// to more than kLimit: the tile is then computed a second time with its maximum.
-// Otherwise no tile needs a maximum, whose cost per score is a third of the
-// exponential's, nor the sums a rescaling; float32 sums and the operand types
-// hold powers of that size as well as those below 1.
-constexpr float kLimit = 4096.f;
+// last set. The scale is set again only when a score is 2^kSlack above it, which
+// each lane sees from its own scores: after a row's first tiles neither the lane
+// exchange of the maximum nor the rescaling of the sums runs (ViT-L training case:
+// 541 us when a tile was computed twice instead, on sums that had grown too large,
+// to save the maximum as well; 497 us so). Powers stay below 2^kSlack, which
+// float32 sums and the operand types hold as well as those below 1.
+constexpr float kSlack = 8.f;
 
 // Keys of a staged tile: 64, or 32 per wave where the waves share a tile.
 template <int WM> constexpr int kTileKeys = WM == 1 ? 128 : 64;
 
 // The keys of one sample and key head as a workgroup walks over them: tiles of
 // TK keys and values in LDS, two of them where they fit (one is read while the
-// next arrives), and which keys are seen.
+// next arrives). With a tile that has unseen keys comes what their scores start
+// from, -inf (0 for the others): as the sum's initial value in the product that
+// makes the scores it costs nothing, and unseen keys and values are zeros.
 template <typename T, int TK, int W, bool VEC>
 struct KeyTiles {
     typedef Stage<T, TK, W, VEC> S;
@@ -44,23 +47,24 @@ struct KeyTiles {
     S sk, sv;
     const T *k, *v;
     const uint8_t* mask;
-    int64_t len, t0, t1;
-    unsigned char* mem;     // [kBuffers][K, V]
-    uint8_t* seen_mem;      // [kBuffers][TK]
+    int64_t len, t0, t1, tw;  // tiles t0 .. t1, of which those below tw are whole
+    unsigned char* mem;       // [kBuffers][K, V]
+    float* start_mem;         // [kBuffers][TK]
     uint8_t next[S::kCount];  // the mask at the next tile's rows
     uint8_t own, own_next;    // and at row threadIdx.x
 
-    __device__ __forceinline__ KeyTiles(const CrossArgs& p, int b, int j, int split, unsigned char* mem, uint8_t* seen_mem)
+    __device__ __forceinline__ KeyTiles(const CrossArgs& p, int b, int j, int split, unsigned char* mem, float* start_mem)
         : k((const T*)p.k + b * p.kb + j * p.kh), v((const T*)p.v + b * p.vb + j * p.vh),
-          mask(p.mask ? p.mask + b * p.mask_b : nullptr), len(seen_length(p, b)), mem(mem), seen_mem(seen_mem) {
+          mask(p.mask ? p.mask + b * p.mask_b : nullptr), len(seen_length(p, b)), mem(mem), start_mem(start_mem) {
         const uint32_t tiles = (uint32_t)cdiv(len, TK), per = (tiles + p.splits - 1) / p.splits;
         t0 = split * per, t1 = lesser(tiles, split * per + per);
+        tw = mask ? t0 : max<int64_t>(t0, lesser<int64_t>(t1, len / TK));
     }
 
     __device__ __forceinline__ int left(int64_t tile) const { return (int)lesser<int64_t>(len - tile * TK, TK); }
     __device__ __forceinline__ unsigned char* keys(int64_t tile) const { return mem + (kBuffers == 2 ? (int)(tile & 1) * kTile : 0); }
     __device__ __forceinline__ unsigned char* values(int64_t tile) const { return keys(tile) + S::kBytes; }
-    __device__ __forceinline__ uint8_t* seen(int64_t tile) const { return seen_mem + (kBuffers == 2 ? (int)(tile & 1) * TK : 0); }
+    __device__ __forceinline__ float* start(int64_t tile) const { return start_mem + (kBuffers == 2 ? (int)(tile & 1) * TK : 0); }
 
     // The mask is read a tile ahead of the rows whose loads depend on it.
     __device__ __forceinline__ void fetch_mask(const CrossArgs& p, int64_t tile) {
@@ -89,7 +93,8 @@ struct KeyTiles {
     }
     template <bool MASK>
     __device__ __forceinline__ void arrive(int64_t tile) {
-        if (MASK && mask && threadIdx.x < TK) seen(tile)[threadIdx.x] = own_next;
+        if (tile >= tw && threadIdx.x < TK)
+            start(tile)[threadIdx.x] = (int)threadIdx.x < left(tile) && (!MASK || !mask || own_next) ? 0.f : kNegInf;
         sk.store(keys(tile));
         sv.store(values(tile));
         landed();
@@ -101,7 +106,6 @@ struct KeyTiles {
     template <typename F, typename G>
     __device__ __forceinline__ void walk(const CrossArgs& p, F whole, G part) {
         if (t0 >= t1) return;
-        const int64_t tw = mask ? t0 : max<int64_t>(t0, lesser(t1, len / TK));
         fetch_mask(p, t0);
         if constexpr (kBuffers == 2) {
             fetch<true>(p, t0);
@@ -126,6 +130,19 @@ struct KeyTiles {
     }
 };
 
+// What the scores of a tile of S keys from `at` on start from
+template <typename M>
+__device__ __forceinline__ typename M::Acc start_scores(const float* at, int lane) {
+    typename M::Acc a;
+#pragma unroll
+    for (int q = 0; q < M::Q; ++q) {
+        const f32x4 v = *(const f32x4*)(at + M::row4(q, lane));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[4 * q + e] = v[e];
+    }
+    return a;
+}
+
 template <typename T, int DP, int WM, int S, bool VEC>
 __global__ __launch_bounds__(256, (kResidentFwd<T, DP>)) void k_cross_fwd(CrossArgs p) {
     typedef Shape<T, S> M;
@@ -135,7 +152,7 @@ __global__ __launch_bounds__(256, (kResidentFwd<T, DP>)) void k_cross_fwd(CrossA
     typedef KeyTiles<T, TK, W, VEC> Keys;
     constexpr size_t kJoin = WK > 1 ? (size_t)WK * ROWS * (DB * S + 2) * 4 : 0;
     __shared__ __attribute__((aligned(16))) unsigned char mem[Keys::kBytes > kJoin ? Keys::kBytes : kJoin];
-    __shared__ __attribute__((aligned(16))) uint8_t seen_mem[Keys::kBuffers * TK];
+    __shared__ __attribute__((aligned(16))) float start_mem[Keys::kBuffers * TK];
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave % WM, wk = wave / WM;
     const int li = M::col(lane), slot = M::slot(lane);
@@ -143,7 +160,7 @@ __global__ __launch_bounds__(256, (kResidentFwd<T, DP>)) void k_cross_fwd(CrossA
     const HeadTile ht = head_tile(blockIdx.x, gridDim.x, row_tiles * p.splits);
     const int j = ht.bh % p.KH, b = sample_of_rank(p, ht.bh / p.KH), bh = b * p.KH + j, split = (int)(ht.tile / row_tiles);
     const int64_t r = (int64_t)(ht.tile - split * row_tiles) * ROWS + wm * S + li;  // this lane's row
-    Keys keys(p, b, j, split, mem, seen_mem);
+    Keys keys(p, b, j, split, mem, start_mem);
 
     Frag8<T> qf[KS];
     {
@@ -158,53 +175,35 @@ __global__ __launch_bounds__(256, (kResidentFwd<T, DP>)) void k_cross_fwd(CrossA
     auto use = [&](int64_t tile, auto part) __attribute__((always_inline)) {
         const unsigned char *const lk = keys.keys(tile), *const lv = keys.values(tile);
         Acc s[NB];
-        float sum;
-        for (bool with_max = __any(m == kNegInf);; with_max = true) {
+        float top = m;
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                s[nb] = M::fill(0.f);
+        for (int nb = 0; nb < NB; ++nb) {
+            if constexpr (part.value) s[nb] = start_scores<M>(keys.start(tile) + wk * KW + nb * S, lane);
+            else s[nb] = M::fill(0.f);
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks)
-                    s[nb] = M::mma(M::template frag<W>(lk, wk * KW + nb * S, ks, lane), qf[ks], s[nb]);
-            }
-            if constexpr (part.value) {
-                const int left = keys.left(tile);
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                    for (int q = 0; q < M::Q; ++q) {
-                        const int at = wk * KW + nb * S + M::row4(q, lane);
-                        const uint32_t w = keys.mask ? *(const uint32_t*)(keys.seen(tile) + at) : 0x01010101u;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            s[nb][4 * q + e] = at + e < left && ((w >> (8 * e)) & 0xff) ? s[nb][4 * q + e] : kNegInf;
-                    }
-            }
-            if (with_max) {
-                float top = m;
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                    for (int e = 0; e < 4 * M::Q; ++e) top = fmaxf(top, s[nb][e]);
-                top = M::col_max(top);
-                const float f = top == kNegInf ? 1.f : __builtin_amdgcn_exp2f((m - top) * p.c);
-                m = top;
-                l *= f;
-#pragma unroll
-                for (int db = 0; db < DB; ++db) acc[db] *= f;
-            }
-            const float mc = m == kNegInf ? 0.f : m * p.c;  // no key seen so far: every power is 0
-            sum = 0.f;
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                for (int e = 0; e < 4 * M::Q; ++e) {
-                    s[nb][e] = __builtin_amdgcn_exp2f(fmaf(s[nb][e], p.c, -mc));
-                    sum += s[nb][e];
-                }
-            if (with_max || !__any(!(sum <= kLimit))) break;
+            for (int ks = 0; ks < KS; ++ks)
+                s[nb] = M::mma(M::template frag<W>(lk, wk * KW + nb * S, ks, lane), qf[ks], s[nb]);
         }
-        l += sum;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int e = 0; e < 4 * M::Q; ++e) top = fmaxf(top, s[nb][e]);
+        if (__any((top - m) * p.c > kSlack)) {
+            top = M::col_max(top);
+            const float f = top == kNegInf ? 1.f : __builtin_amdgcn_exp2f((m - top) * p.c);
+            m = top;
+            l *= f;
+#pragma unroll
+            for (int db = 0; db < DB; ++db) acc[db] *= f;
+        }
+        const float mc = m == kNegInf ? 0.f : m * p.c;  // no key seen so far: every power is 0
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int e = 0; e < 4 * M::Q; ++e) {
+                s[nb][e] = __builtin_amdgcn_exp2f(fmaf(s[nb][e], p.c, -mc));
+                l += s[nb][e];
+            }
 #pragma unroll
         for (int kk = 0; kk < KW / M::K; ++kk) {
             const Frag8<T> pf = M::pack(s, kk);

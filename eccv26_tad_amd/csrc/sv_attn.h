@@ -316,6 +316,7 @@ struct CrossArgs {
     int splits;            // of the reduced axis
     float c, scale;        // c = scale log2(e)
     float inv_g;           // 1 / G
+    float up, down;        // a power of two and its inverse: what float16 probabilities are scaled by in dv
     bool vec;              // D and all strides are multiples of 8 elements, all starts of 16 bytes
 };
 

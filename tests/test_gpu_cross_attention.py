@@ -103,6 +103,12 @@ def test_split_axes(dev, Nq, Nk, dtype):
     _check(*_inputs(dev, 1, Nq, Nk, 2, 2, 64, DTYPES[dtype]))
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_probabilities_below_the_types_normal_range(dev, dtype):
+    """Among 20000 keys a probability is 5e-5, below float16's normal values."""
+    _check(*_inputs(dev, 1, 70, 20000, 2, 2, 32, DTYPES[dtype]))
+
+
 @pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
 @pytest.mark.parametrize("Nq,Nk", [(1, 700), (20, 200), (150, 130)])
 @pytest.mark.parametrize("kind", ["lengths", "mask", "both"])

@@ -7,7 +7,7 @@
 namespace svtad {
 
 constexpr int kMaxHeadDim = 128;
-constexpr int kWantGroups = 512;  // two workgroups per compute unit
+constexpr int kWantGroups = 512;  // two workgroups per compute unit, and not a few more, which would run alone
 constexpr int kMaxSplits = 64;  // k_cross_join holds a quarter of them in registers
 
 // How a kernel over row tiles (forward, dq) is cut: waves along the rows, and
@@ -24,7 +24,7 @@ static RowPlan row_plan(const svtad_cross_args& a) {
     const int64_t rows = r.wave_rows == 4 ? 128 : r.wave_rows == 2 ? 64 : 16;
     const int64_t groups = std::max<int64_t>(1, cdiv(m, rows) * a.batch * a.kv_heads);
     const int64_t tiles = cdiv(a.nk, r.wave_rows == 1 ? 128 : 64);
-    r.splits = (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(kWantGroups, groups), tiles / 2, (int64_t)kMaxSplits}));
+    r.splits = (int)std::max<int64_t>(1, std::min<int64_t>({kWantGroups / groups, tiles / 2, (int64_t)kMaxSplits}));
     return r;
 }
 
@@ -32,7 +32,7 @@ static RowPlan row_plan(const svtad_cross_args& a) {
 static int key_plan(const svtad_cross_args& a) {
     const int64_t m = a.nq * (a.heads / a.kv_heads);
     const int64_t groups = std::max<int64_t>(1, cdiv(a.nk, kCrossKvKeys) * a.batch * a.kv_heads);
-    return (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(kWantGroups, groups), cdiv(m, 64) / 2, (int64_t)kMaxSplits}));
+    return (int)std::max<int64_t>(1, std::min<int64_t>({kWantGroups / groups, cdiv(m, 64) / 2, (int64_t)kMaxSplits}));
 }
 
 static size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }

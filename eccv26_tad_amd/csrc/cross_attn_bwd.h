@@ -76,9 +76,11 @@ __global__ __launch_bounds__(256, (kResidentBwd<T, DP>)) void k_cross_bwd_q(Cros
                 if constexpr (part.value) s = start_scores<M>(keys.start(tile) + row, lane);
                 else s = M::fill(0.f);
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) s = M::mma(M::template frag<W>(lk, row, ks, lane), qf[ks], s);
+                for (int ks = 0; ks < KS; ++ks)
+                    if (M::step_in(ks, p.D)) s = M::mma(M::template frag<W>(lk, row, ks, lane), qf[ks], s);
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) dp = M::mma(M::template frag<W>(lv, row, ks, lane), df[ks], dp);
+                for (int ks = 0; ks < KS; ++ks)
+                    if (M::step_in(ks, p.D)) dp = M::mma(M::template frag<W>(lv, row, ks, lane), df[ks], dp);
 #pragma unroll
                 for (int e = 0; e < 4 * M::Q; ++e) ds[h][e] = __builtin_amdgcn_exp2f(fmaf(s[e], p.c, -lse)) * dp[e];
             }
@@ -224,9 +226,11 @@ __global__ __launch_bounds__(256, (kResidentBwd<T, DP>)) void k_cross_bwd_kv(Cro
                 for (int e = 0; e < 4; ++e) dp[4 * q + e] = d4[e];  // -delta: the product's own sum is dp - delta
             }
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) s = M::mma(M::template frag<W>(lq, row, ks, lane), kf[ks], s);
+            for (int ks = 0; ks < KS; ++ks)
+                if (M::step_in(ks, p.D)) s = M::mma(M::template frag<W>(lq, row, ks, lane), kf[ks], s);
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) dp = M::mma(M::template frag<W>(ld, row, ks, lane), vf[ks], dp);
+            for (int ks = 0; ks < KS; ++ks)
+                if (M::step_in(ks, p.D)) dp = M::mma(M::template frag<W>(ld, row, ks, lane), vf[ks], dp);
 #pragma unroll
             for (int q = 0; q < M::Q; ++q) {
                 const f32x4 l4 = *(const f32x4*)(l_tile + row + M::row4(q, lane));

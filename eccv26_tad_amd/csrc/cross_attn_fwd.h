@@ -39,9 +39,9 @@ template <int WM> constexpr int kTileKeys = WM == 1 ? 128 : 64;
 // next arrives). With a tile that has unseen keys comes what their scores start
 // from, -inf (0 for the others): as the sum's initial value in the product that
 // makes the scores it costs nothing, and unseen keys and values are zeros.
-template <typename T, int TK, int W, bool VEC>
+template <typename T, int TK, int W, bool VEC, bool ONCE = false>
 struct KeyTiles {
-    typedef Stage<T, TK, W, VEC> S;
+    typedef Stage<T, TK, W, VEC, ONCE> S;
     static constexpr int kTile = 2 * S::kBytes, kBuffers = 2 * kTile <= 128 * 1024 ? 2 : 1;
     static constexpr size_t kBytes = (size_t)kBuffers * kTile;
     S sk, sv;
@@ -149,7 +149,9 @@ __global__ __launch_bounds__(256, (kResidentFwd<T, DP>)) void k_cross_fwd(CrossA
     typedef typename M::Acc Acc;
     constexpr int W = DP < 32 ? 32 : DP, KS = W / M::K, DB = DP < S ? 1 : DP / S;
     constexpr int WK = 4 / WM, TK = kTileKeys<WM>, KW = TK / WK, NB = KW / S, ROWS = WM * S;
-    typedef KeyTiles<T, TK, W, VEC> Keys;
+    // Up to 16 rows (WM 1) are one row tile: each key is read by one workgroup (8 x
+    // 31361 keys, one query each, a pass: 40.7 us past the caches, 44.0 through).
+    typedef KeyTiles<T, TK, W, VEC, WM == 1> Keys;
     constexpr size_t kJoin = WK > 1 ? (size_t)WK * ROWS * (DB * S + 2) * 4 : 0;
     __shared__ __attribute__((aligned(16))) unsigned char mem[Keys::kBytes > kJoin ? Keys::kBytes : kJoin];
     __shared__ __attribute__((aligned(16))) float start_mem[Keys::kBuffers * TK];
@@ -182,7 +184,7 @@ __global__ __launch_bounds__(256, (kResidentFwd<T, DP>)) void k_cross_fwd(CrossA
             else s[nb] = M::fill(0.f);
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
-                s[nb] = M::mma(M::template frag<W>(lk, wk * KW + nb * S, ks, lane), qf[ks], s[nb]);
+                if (M::step_in(ks, p.D)) s[nb] = M::mma(M::template frag<W>(lk, wk * KW + nb * S, ks, lane), qf[ks], s[nb]);
         }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)

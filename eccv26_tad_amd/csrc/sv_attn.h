@@ -103,6 +103,9 @@ struct Shape {
             return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a.v), __builtin_bit_cast(bf16x8, b.v), c, 0, 0, 0);
         }
     }
+    // Whether product ks of a row of d elements has any: float32 products are slow
+    // enough for the branch, in 16 bits the zeros are multiplied.
+    static __device__ __forceinline__ bool step_in(int ks, int d) { return sizeof(T) == 2 || ks * K < d; }
     static __device__ __forceinline__ Acc fill(float v) {
         Acc a;
 #pragma unroll
@@ -230,12 +233,20 @@ __device__ __forceinline__ uint32_t lds_offset(const void* p) {
 // tell which of two tiles they go to, and no load would be in flight during the
 // work on the tile before. There is no output register; `landed` waits. m0, which
 // holds the LDS address, is set in the same statement and holds nothing else here.
+// ONCE: memory that nobody reads again, not kept in the caches.
+template <bool ONCE>
 __device__ __forceinline__ void load_to_lds(u32x4 r, uint32_t offset, const unsigned char* to) {
     const uint32_t base = lds_offset(to);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                 :
-                 : "s"(base), "v"(offset), "s"(r)
-                 : "memory");
+    if constexpr (ONCE)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds"
+                     :
+                     : "s"(base), "v"(offset), "s"(r)
+                     : "memory");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                     :
+                     : "s"(base), "v"(offset), "s"(r)
+                     : "memory");
 }
 
 // The same for 4 bytes per lane.
@@ -252,7 +263,7 @@ __device__ __forceinline__ void load_word_to_lds(u32x4 r, uint32_t offset, const
 // zeros without a branch. VEC: straight to LDS, without registers; a barrier
 // after `landed` makes the tile readable. Otherwise element by element through
 // registers, which `store` empties into the tile.
-template <typename T, int TILE, int W, bool VEC>
+template <typename T, int TILE, int W, bool VEC, bool ONCE = false>
 struct Stage {
     typedef LdsTile<T, W> Tile;
     static constexpr int kCount = TILE * Tile::kPieces / 256, kBytes = TILE * Tile::kRow, E = Tile::kElems;
@@ -269,7 +280,7 @@ struct Stage {
         constexpr int S = (int)sizeof(T);
         const int c = col(i);
         if constexpr (VEC) {
-            load_to_lds(r.q, c < d ? at + c * S : kOOB, tile + (i * 256 + (threadIdx.x & ~63)) * 16);
+            load_to_lds<ONCE>(r.q, c < d ? at + c * S : kOOB, tile + (i * 256 + (threadIdx.x & ~63)) * 16);
         } else {
             Pack<T, E> p;
 #pragma unroll

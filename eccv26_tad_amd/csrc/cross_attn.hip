@@ -120,7 +120,7 @@ extern "C" size_t svtad_cross_attention_bwd_workspace_bytes(const svtad_cross_ar
     return cross_check(a, dtype) ? 0 : bwd_bytes(*a);
 }
 
-extern "C" int svtad_cross_attention(const svtad_cross_args* a, void* out, float* lse, void* workspace,
+extern "C" int svtad_cross_attention(const svtad_cross_args* a, void* out, float* lse, void* rest, void* workspace,
                                      size_t workspace_bytes, int dtype, void* stream) {
     const int st = cross_check(a, dtype);
     if (st) return st;
@@ -131,7 +131,7 @@ extern "C" int svtad_cross_attention(const svtad_cross_args* a, void* out, float
         return set_error(SVTAD_ERR_WORKSPACE, "cross_attention: workspace too small");
     const RowPlan plan = row_plan(*a);
     CrossArgs p = cross_args(*a, dtype);
-    p.out = out, p.lse = lse;
+    p.out = out, p.lse = lse, p.rest = dtype == SVTAD_F32 ? nullptr : rest;
     p.splits = plan.splits, p.part = (float*)workspace;
     if (dtype == SVTAD_F16) cross_fwd<f16>(p, plan.wave_rows, (hipStream_t)stream);
     else if (dtype == SVTAD_BF16) cross_fwd<bf16>(p, plan.wave_rows, (hipStream_t)stream);
@@ -153,8 +153,8 @@ static void cross_bwd(CrossArgs p, const svtad_cross_args& a, hipStream_t st) {
     }
 }
 
-extern "C" int svtad_cross_attention_bwd(const svtad_cross_args* a, const void* out, const float* lse, const void* dout,
-                                         const int64_t* dout_stride, void* dq, void* dk, void* dv, void* workspace,
+extern "C" int svtad_cross_attention_bwd(const svtad_cross_args* a, const void* out, const void* rest, const float* lse,
+                                         const void* dout, const int64_t* dout_stride, void* dq, void* dk, void* dv, void* workspace,
                                          size_t workspace_bytes, int dtype, void* stream) {
     const int st = cross_check(a, dtype);
     if (st) return st;
@@ -166,11 +166,12 @@ extern "C" int svtad_cross_attention_bwd(const svtad_cross_args* a, const void* 
     if (need && (!workspace || workspace_bytes < need))
         return set_error(SVTAD_ERR_WORKSPACE, "cross_attention_bwd: workspace too small");
     CrossArgs p = cross_args(*a, dtype);
+    p.rest = dtype == SVTAD_F32 ? nullptr : const_cast<void*>(rest);
     p.o = out, p.on = (int64_t)a->heads * a->head_dim, p.oh = a->head_dim, p.ob = a->nq * p.on;
     p.dout = dout;
     if (dout_stride && !near_strides(dout_stride, p.G, dtype))
         return set_error(SVTAD_ERR_UNSUPPORTED, "cross_attention_bwd: 128 tokens of dout must lie within 2 GiB");
-    p.vec = p.vec && (uintptr_t)out % 16 == 0 && (!dout_stride || whole_vectors(*a, dout, dout_stride, a->nq, a->heads));
+    p.vec = p.vec && (uintptr_t)out % 16 == 0 && (uintptr_t)p.rest % 16 == 0 && (!dout_stride || whole_vectors(*a, dout, dout_stride, a->nq, a->heads));
     if (dout_stride) p.gb = dout_stride[0], p.gn = dout_stride[1], p.gh = dout_stride[2];
     p.out = dq, p.dk = dk, p.dv = dv;
     p.lse = const_cast<float*>(lse);

@@ -278,12 +278,14 @@ __global__ __launch_bounds__(256, (kResidentFwd<T, DP>)) void k_cross_fwd(CrossA
         }
         return;
     }
-    T* const o = (T*)p.out + (int64_t)b * p.Nq * p.H * p.D + row_at(p, r, (int64_t)p.H * p.D, p.D, j);
+    const int64_t o = (int64_t)b * p.Nq * p.H * p.D + row_at(p, r, (int64_t)p.H * p.D, p.D, j);
     const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
-        for (int q = 0; q < M::Q; ++q) store4<T>(o, db * S + M::row4(q, lane), p.D, M::quad(acc[db], q) * inv);
+        for (int q = 0; q < M::Q; ++q)
+            store4_rest<T>((T*)p.out + o, p.rest ? (T*)p.rest + o : nullptr, db * S + M::row4(q, lane), p.D,
+                           M::quad(acc[db], q) * inv);
     if (p.lse && slot == 0) p.lse[bh * p.M + r] = l == 0.f ? -kNegInf : m * p.c + __builtin_amdgcn_logf(l);
 }
 
@@ -333,8 +335,8 @@ __global__ __launch_bounds__(256) void k_cross_join(CrossArgs p) {
     for (int q = 1; q < kJoinGroups; ++q) l += red[q][chunk][1];
     const int64_t bh = at / p.M, r = at - bh * p.M, b = bh / p.KH;
     const int j = (int)(bh - b * p.KH);
-    T* const o = (T*)p.out + b * p.Nq * p.H * p.D + row_at(p, r, (int64_t)p.H * p.D, p.D, j);
-    store4<T>(o, c, p.D, acc * (l == 0.f ? 0.f : 1.f / l));
+    const int64_t o = b * p.Nq * p.H * p.D + row_at(p, r, (int64_t)p.H * p.D, p.D, j);
+    store4_rest<T>((T*)p.out + o, p.rest ? (T*)p.rest + o : nullptr, c, p.D, acc * (l == 0.f ? 0.f : 1.f / l));
     if (p.lse && c == 0) p.lse[at] = l == 0.f ? -kNegInf : top * p.c + __builtin_amdgcn_logf(l);
 }
 

@@ -208,6 +208,17 @@ __device__ __forceinline__ void store4(T* row, int c, int d, f32x4 v) {
     }
 }
 
+// Stores 4 values as T, and with `rest` what the rounding took from them, as T
+template <typename T>
+__device__ __forceinline__ void store4_rest(T* row, T* rest, int c, int d, f32x4 v) {
+    store4<T>(row, c, d, v);
+    if (rest) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] -= (float)(T)v[e];
+        store4<T>(rest, c, d, v);
+    }
+}
+
 // A buffer from `base` (the same for the wave) on, as the builtins and as the
 // instruction take it. Loads check their rows themselves and give kOOB where
 // there is none; valid offsets are below 2^31.
@@ -315,6 +326,7 @@ __device__ __forceinline__ void landed() {
 struct CrossArgs {
     const void *q, *k, *v, *o, *dout;
     void *out, *dk, *dv;   // out: the forward's output, or dq
+    void* rest;            // like the forward's output: what its rounding took (NULL: not kept)
     float* lse;            // [B KH][M]: log2 of a row's sum of 2^(c s), +inf for a row that sees no key
     float* delta;          // [B KH][M]: minus the sum over d of dout out
     const int32_t* lengths;   // [B] or NULL

@@ -215,35 +215,39 @@ CrossCall cross_call(const at::Tensor& q, const at::Tensor& k, const at::Tensor&
 
 }  // namespace
 
-// cross_attention(q, k, v, key_lengths, key_mask, scale, want_lse) -> (out, lse: one float32 per row, for the backward, or empty)
-std::tuple<at::Tensor, at::Tensor> op_cross_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-                                                      const c10::optional<at::Tensor>& lengths,
-                                                      const c10::optional<at::Tensor>& mask, double scale, bool want_lse) {
+// cross_attention(q, k, v, key_lengths, key_mask, scale, train) -> (out, lse, rest): for the backward one float32
+// per row and what the output's rounding took, or empty
+std::tuple<at::Tensor, at::Tensor, at::Tensor> op_cross_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                                  const c10::optional<at::Tensor>& lengths,
+                                                                  const c10::optional<at::Tensor>& mask, double scale,
+                                                                  bool train) {
     CrossCall c = cross_call(q, k, v, lengths, mask, scale, "cross_attention");
     c10::DeviceGuard g(q.device());
     const int dt = dtype_code(q);
-    at::Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
-    at::Tensor lse = at::empty({want_lse ? q.size(0) : 0, q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
+    at::Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous)), lse, rest;
+    if (train) lse = at::empty({q.size(0), q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
+    if (train && q.scalar_type() != at::kFloat) rest = at::empty_like(out);
     const size_t bytes = svtad_cross_attention_workspace_bytes(&c.a, dt);
     at::Tensor ws = workspace(bytes, q);
-    check_status(svtad_cross_attention(&c.a, out.data_ptr(), want_lse ? lse.data_ptr<float>() : nullptr, ptr(ws), bytes, dt,
-                                       stream_of(q)),
+    check_status(svtad_cross_attention(&c.a, out.data_ptr(), (float*)ptr(lse), ptr(rest), ptr(ws), bytes, dt, stream_of(q)),
                  "cross_attention");
-    return {out, lse};
+    return {out, lse, rest};
 }
 
-// cross_attention_bwd(dout, q, k, v, out, lse, key_lengths, key_mask, scale, need_q, need_kv) -> (dq, dk, dv)
+// cross_attention_bwd(dout, q, k, v, out, lse, rest (or None), key_lengths, key_mask, scale, need_q, need_kv) -> (dq, dk, dv)
 std::tuple<at::Tensor, at::Tensor, at::Tensor> op_cross_attention_bwd(
     const at::Tensor& dout_in, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& out,
-    const at::Tensor& lse, const c10::optional<at::Tensor>& lengths, const c10::optional<at::Tensor>& mask, double scale,
-    bool need_q, bool need_kv) {
+    const at::Tensor& lse, const c10::optional<at::Tensor>& rest, const c10::optional<at::Tensor>& lengths,
+    const c10::optional<at::Tensor>& mask, double scale, bool need_q, bool need_kv) {
     CrossCall c = cross_call(q, k, v, lengths, mask, scale, "cross_attention_bwd");
-    for (const at::Tensor* t : {&dout_in, &out})
+    const bool has_rest = rest.has_value() && rest->defined();
+    for (const at::Tensor* t : {&dout_in, &out, has_rest ? &*rest : &out})
         TORCH_CHECK(t->sizes() == q.sizes() && t->scalar_type() == q.scalar_type() && t->device() == q.device(),
-                    "opentad_sparse_ops.cross_attention_bwd: dout and out must be like q");
-    TORCH_CHECK(out.is_contiguous() && lse.is_contiguous() && lse.scalar_type() == at::kFloat &&
-                    lse.numel() == q.size(0) * q.size(1) * q.size(2) && lse.device() == q.device(),
-                "opentad_sparse_ops.cross_attention_bwd: out and lse must be the forward's");
+                    "opentad_sparse_ops.cross_attention_bwd: dout, out and rest must be like q");
+    TORCH_CHECK(out.is_contiguous() && (!has_rest || rest->is_contiguous()) && lse.is_contiguous() &&
+                    lse.scalar_type() == at::kFloat && lse.numel() == q.size(0) * q.size(1) * q.size(2) &&
+                    lse.device() == q.device(),
+                "opentad_sparse_ops.cross_attention_bwd: out, lse and rest must be the forward's");
     c10::DeviceGuard g(q.device());
     const int dt = dtype_code(q);
     const at::Tensor dout = readable(dout_in, q.size(2) / k.size(2));
@@ -254,8 +258,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> op_cross_attention_bwd(
     if (need_kv) dk = dense(k), dv = dense(v);
     const size_t bytes = svtad_cross_attention_bwd_workspace_bytes(&c.a, dt);
     at::Tensor ws = workspace(bytes, q);
-    check_status(svtad_cross_attention_bwd(&c.a, out.data_ptr(), lse.data_ptr<float>(), dout.data_ptr(), ds, ptr(dq), ptr(dk),
-                                           ptr(dv), ptr(ws), bytes, dt, stream_of(q)),
+    check_status(svtad_cross_attention_bwd(&c.a, out.data_ptr(), ptr(rest), lse.data_ptr<float>(), dout.data_ptr(), ds,
+                                           ptr(dq), ptr(dk), ptr(dv), ptr(ws), bytes, dt, stream_of(q)),
                  "cross_attention_bwd");
     return {dq, dk, dv};
 }
@@ -313,18 +317,22 @@ namespace {
 
 // The autograd nodes. They are written here and not in Python because a small
 // layer's backward is host time: the engine's thread then needs no interpreter
-// (64 x 32 rows of layer norm, forward and backward: 91 us with a Python node).
+// (64 x 32 rows of layer norm, forward and backward: 68 us, 91 with a Python node).
 
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
 // Gradients of a node that is differentiable once: a second derivative raises.
-variable_list once(variable_list grads, const char* who) {
+// The gradients hang on all they were made `from`, so that no path to those is
+// left out in silence.
+variable_list once(variable_list grads, const variable_list& from, const char* who) {
     if (!at::GradMode::is_enabled()) return grads;
     variable_list given;
     for (const auto& g : grads)
         if (g.defined()) given.push_back(g.detach().requires_grad_(true));
     if (given.empty()) return grads;
+    for (const auto& t : from)
+        if (t.defined()) given.push_back(t);
     auto error = std::make_shared<torch::autograd::DelayedError>(
         std::string("trying to differentiate ") + who + " twice", (int64_t)given.size());
     given = (*error)(std::move(given));
@@ -365,7 +373,7 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
             std::tie(dx, dw, db) = op_layer_norm_bwd(dy[0], saved[0], saved[1], has_w ? c10::make_optional(saved[2]) : c10::nullopt,
                                                      ctx->saved_data["f32"].toBool(), need_x, need_w, need_b);
         }
-        variable_list g = once({dx, dw, db}, "layer_norm");
+        variable_list g = once({dx, dw, db}, {dy[0], saved[0], saved[2]}, "layer_norm");
         g.emplace_back();
         return g;
     }
@@ -374,9 +382,9 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
 struct CrossAttentionNode : torch::autograd::Function<CrossAttentionNode> {
     static at::Tensor forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                               const c10::optional<at::Tensor>& lengths, const c10::optional<at::Tensor>& mask, double scale) {
-        at::Tensor out, lse;
-        std::tie(out, lse) = op_cross_attention(q, k, v, lengths, mask, scale, true);
-        ctx->save_for_backward({q, k, v, out, lse, lengths.value_or(at::Tensor()), mask.value_or(at::Tensor())});
+        at::Tensor out, lse, rest;
+        std::tie(out, lse, rest) = op_cross_attention(q, k, v, lengths, mask, scale, true);
+        ctx->save_for_backward({q, k, v, out, lse, rest, lengths.value_or(at::Tensor()), mask.value_or(at::Tensor())});
         ctx->saved_data["scale"] = scale;
         return out;
     }
@@ -388,9 +396,11 @@ struct CrossAttentionNode : torch::autograd::Function<CrossAttentionNode> {
             at::NoGradGuard guard;
             const auto given = [](const at::Tensor& t) { return t.defined() ? c10::make_optional(t) : c10::nullopt; };
             std::tie(dq, dk, dv) = op_cross_attention_bwd(dout[0], s[0], s[1], s[2], s[3], s[4], given(s[5]), given(s[6]),
+                                                          given(s[7]),
                                                           ctx->saved_data["scale"].toDouble(), need_q, need_k || need_v);
         }
-        variable_list g = once({dq, need_k ? dk : at::Tensor(), need_v ? dv : at::Tensor()}, "cross_attention");
+        variable_list g = once({dq, need_k ? dk : at::Tensor(), need_v ? dv : at::Tensor()},
+                               {dout[0], s[0], s[1], s[2]}, "cross_attention");
         g.resize(6);
         return g;
     }
@@ -416,13 +426,13 @@ void bind_operators(pybind11::module& m) {
           py::arg("bias"), py::arg("eps"));
     m.def("layer_norm_bwd", &op_layer_norm_bwd, "Its gradients (dx, dw, db)", py::arg("dy"), py::arg("x"), py::arg("stats"),
           py::arg("weight"), py::arg("params_f32"), py::arg("need_x"), py::arg("need_w"), py::arg("need_b"));
-    m.def("cross_attention", &op_cross_attention, "Attention of queries to the keys of another sequence (out, lse)",
+    m.def("cross_attention", &op_cross_attention, "Attention of queries to the keys of another sequence (out, lse, rest)",
           py::arg("q"), py::arg("k"), py::arg("v"), py::arg("key_lengths"), py::arg("key_mask"), py::arg("scale"),
-          py::arg("want_lse"));
+          py::arg("train"));
     m.def("cross_attention_grad", &op_cross_attention_grad, "cross_attention as a differentiable function", py::arg("q"),
           py::arg("k"), py::arg("v"), py::arg("key_lengths"), py::arg("key_mask"), py::arg("scale"));
     m.def("cross_attention_bwd", &op_cross_attention_bwd, "Its gradients (dq, dk, dv)", py::arg("dout"), py::arg("q"),
-          py::arg("k"), py::arg("v"), py::arg("out"), py::arg("lse"), py::arg("key_lengths"), py::arg("key_mask"),
+          py::arg("k"), py::arg("v"), py::arg("out"), py::arg("lse"), py::arg("rest"), py::arg("key_lengths"), py::arg("key_mask"),
           py::arg("scale"), py::arg("need_q"), py::arg("need_kv"));
     m.def("grad_clip", &op_grad_clip, "The norm over all gradients, and the gradients scaled down to a limit",
           py::arg("grads"), py::arg("outs"), py::arg("write"), py::arg("max_norm"), py::arg("scale"), py::arg("inf"));

@@ -702,8 +702,9 @@ int svtad_norm_bwd(const svtad_norm_args* args, const void* dy, void* dx, void* 
  * (NULL: all). out [batch, nq, heads, head_dim] is dense. A row that sees no
  * key is 0 and has no gradient; what lies in unseen keys is never used.
  * head_dim is 1 to 128, scale is positive. lse [batch, kv_heads, nq * heads /
- * kv_heads] (NULL: not kept) is what the backward needs beside out. dq, dk, dv
- * are dense; dq may be NULL, dk and dv both. Sums and softmax statistics are
+ * kv_heads] (NULL: not kept) is what the backward needs beside out; rest, like
+ * out (NULL: not kept), is what out's rounding to 16 bits took, for a more exact
+ * backward (not used in float32). dq, dk, dv are dense; dq may be NULL, dk and dv both. Sums and softmax statistics are
  * float32 in a fixed order; probabilities and score gradients are rounded to
  * dtype as operands of the matrix units.
  */
@@ -719,12 +720,12 @@ typedef struct {
     float scale;
 } svtad_cross_args;
 size_t svtad_cross_attention_workspace_bytes(const svtad_cross_args* args, int dtype);
-int svtad_cross_attention(const svtad_cross_args* args, void* out, float* lse, void* workspace, size_t workspace_bytes,
-                          int dtype, void* stream);
+int svtad_cross_attention(const svtad_cross_args* args, void* out, float* lse, void* rest, void* workspace,
+                          size_t workspace_bytes, int dtype, void* stream);
 size_t svtad_cross_attention_bwd_workspace_bytes(const svtad_cross_args* args, int dtype);
-int svtad_cross_attention_bwd(const svtad_cross_args* args, const void* out, const float* lse, const void* dout,
-                              const int64_t* dout_stride, void* dq, void* dk, void* dv, void* workspace,
-                              size_t workspace_bytes, int dtype, void* stream);
+int svtad_cross_attention_bwd(const svtad_cross_args* args, const void* out, const void* rest, const float* lse,
+                              const void* dout, const int64_t* dout_stride, void* dq, void* dk, void* dv,
+                              void* workspace, size_t workspace_bytes, int dtype, void* stream);
 
 /*
  * Gradient clipping over `count` tensors (host array of descriptors; dense

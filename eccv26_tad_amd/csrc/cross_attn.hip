@@ -7,45 +7,68 @@
 namespace svtad {
 
 constexpr int kMaxHeadDim = 128;
-constexpr int kWantGroups = 512;  // two workgroups per compute unit, and not a few more, which would run alone
-constexpr int kMaxSplits = 64;  // k_cross_join holds a quarter of them in registers
+
+// Splits of an axis of `tiles` tiles for `groups` workgroups of `rows` results:
+// as many as fill one, two, three or four workgroups per compute unit, or none,
+// whichever is estimated to take least. The estimate is in times of one tile on a
+// compute unit of its own, 0.87 us in bfloat16 at a head dimension of 64. Two and
+// more workgroups share a unit and take 0.75 of it each, unless one fills it:
+// float32 and wide heads, whose tiles take twice as long as well. Partial results
+// cost a launch (5) and their writing, reading and adding (0.03 for 128 rows of
+// 64). Measured there, 1000 rows, forward, split against whole: 48 groups over 1500
+// keys 17.5 us in four against 25.9, 192 over 500 keys 23.8 in two against 12.3, 192
+// over 20000 keys 176 in four against 202 in two and 277. One query over 8 x 31361
+// keys of 4 heads: 47.3 us in 16, 53.5 in 8, 55.1 in 24. Of 222 kernels at 74 drawn
+// sizes of all types 6 took over 15 % more than in the best of 14 splits (34 % most).
+static int splits(const svtad_cross_args& a, int dtype, int64_t groups, int64_t tiles, int rows) {
+    const bool alone = dtype == SVTAD_F32 || a.head_dim > 64;
+    const double launch = alone ? 2.5 : 5, part = (alone ? 0.015 : 0.03) * rows * a.head_dim / (128 * 64);
+    int best = 1;
+    double least = (double)tiles * (double)cdiv(groups, 256);
+    for (int rounds = 1; rounds <= 4 && groups > 0; ++rounds) {
+        const int64_t most = std::min<int64_t>({256 * rounds / groups, tiles, (int64_t)kMaxSplits});
+        if (most < 2) continue;
+        const int64_t each = cdiv(tiles, most), s = cdiv(tiles, each);  // no more splits than these tiles each need
+        const double time = (double)each * rounds * (rounds == 1 || alone ? 1 : 0.75) + launch + part * (double)(groups * s);
+        if (time < least) best = (int)s, least = time;
+    }
+    return best;
+}
 
 // How a kernel over row tiles (forward, dq) is cut: waves along the rows, and
 // splits of the keys. Rows are not padded to more than twice their number where
-// fewer waves can hold them; the keys are split while there are fewer row
-// tiles than the chip takes at once, into parts of at least two staged tiles.
+// fewer waves can hold them (bfloat16, 8 samples of 16 heads over 8192 keys: 48 us
+// by 64 rows a workgroup against 75 by 16 at 17 rows, 74 against 57 by 128 at 65;
+// float32, one row: 98 us by 16 against 157 by 64 and 312 by 128).
 struct RowPlan {
     int wave_rows, splits;
 };
 
-static RowPlan row_plan(const svtad_cross_args& a) {
+static RowPlan row_plan(const svtad_cross_args& a, int dtype) {
     const int64_t m = a.nq * (a.heads / a.kv_heads);
     RowPlan r{m <= 16 ? 1 : m <= 64 ? 2 : 4, 1};
-    const int64_t rows = r.wave_rows == 4 ? 128 : r.wave_rows == 2 ? 64 : 16;
-    const int64_t groups = std::max<int64_t>(1, cdiv(m, rows) * a.batch * a.kv_heads);
-    const int64_t tiles = cdiv(a.nk, r.wave_rows == 1 ? 128 : 64);
-    r.splits = (int)std::max<int64_t>(1, std::min<int64_t>({kWantGroups / groups, tiles / 2, (int64_t)kMaxSplits}));
+    const int rows = r.wave_rows == 4 ? 128 : r.wave_rows == 2 ? 64 : 16;
+    r.splits = splits(a, dtype, cdiv(m, rows) * a.batch * a.kv_heads, cdiv(a.nk, r.wave_rows == 1 ? 128 : 64), rows);
     return r;
 }
 
 // Splits of the rows in the kernel over key tiles.
-static int key_plan(const svtad_cross_args& a) {
+static int key_plan(const svtad_cross_args& a, int dtype) {
     const int64_t m = a.nq * (a.heads / a.kv_heads);
-    const int64_t groups = std::max<int64_t>(1, cdiv(a.nk, kCrossKvKeys) * a.batch * a.kv_heads);
-    return (int)std::max<int64_t>(1, std::min<int64_t>({kWantGroups / groups, cdiv(m, 64) / 2, (int64_t)kMaxSplits}));
+    return splits(a, dtype, cdiv(a.nk, kCrossKvKeys) * a.batch * a.kv_heads, cdiv(m, 64), kCrossKvKeys);
 }
 
 static size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 static int64_t all_rows(const svtad_cross_args& a) { return a.batch * a.heads * a.nq; }
 static int64_t pad4(int d) { return (d + 3) & ~3; }
 
-static size_t fwd_bytes(const svtad_cross_args& a) {
-    const int s = row_plan(a).splits;
+static size_t fwd_bytes(const svtad_cross_args& a, int dtype) {
+    const int s = row_plan(a, dtype).splits;
     return s > 1 ? (size_t)s * all_rows(a) * (pad4(a.head_dim) + 2) * 4 : 0;
 }
 
-static size_t bwd_bytes(const svtad_cross_args& a) {
-    const int sq = row_plan(a).splits, sk = key_plan(a);
+static size_t bwd_bytes(const svtad_cross_args& a, int dtype) {
+    const int sq = row_plan(a, dtype).splits, sk = key_plan(a, dtype);
     const size_t pq = sq > 1 ? (size_t)sq * all_rows(a) * pad4(a.head_dim) * 4 : 0;
     const size_t pk = sk > 1 ? (size_t)sk * 2 * a.batch * a.kv_heads * a.nk * pad4(a.head_dim) * 4 : 0;
     return align256((size_t)all_rows(a) * 4) + std::max(pq, pk);
@@ -113,11 +136,11 @@ static CrossArgs cross_args(const svtad_cross_args& a, int dtype) {
 using namespace svtad;
 
 extern "C" size_t svtad_cross_attention_workspace_bytes(const svtad_cross_args* a, int dtype) {
-    return cross_check(a, dtype) ? 0 : fwd_bytes(*a);
+    return cross_check(a, dtype) ? 0 : fwd_bytes(*a, dtype);
 }
 
 extern "C" size_t svtad_cross_attention_bwd_workspace_bytes(const svtad_cross_args* a, int dtype) {
-    return cross_check(a, dtype) ? 0 : bwd_bytes(*a);
+    return cross_check(a, dtype) ? 0 : bwd_bytes(*a, dtype);
 }
 
 extern "C" int svtad_cross_attention(const svtad_cross_args* a, void* out, float* lse, void* rest, void* workspace,
@@ -126,10 +149,10 @@ extern "C" int svtad_cross_attention(const svtad_cross_args* a, void* out, float
     if (st) return st;
     if (all_rows(*a) == 0) return SVTAD_OK;
     if (!a->q || !out || (a->nk > 0 && (!a->k || !a->v))) return set_error(SVTAD_ERR_INVALID, "cross_attention: NULL pointer");
-    const size_t need = fwd_bytes(*a);
+    const size_t need = fwd_bytes(*a, dtype);
     if (need && (!workspace || workspace_bytes < need))
         return set_error(SVTAD_ERR_WORKSPACE, "cross_attention: workspace too small");
-    const RowPlan plan = row_plan(*a);
+    const RowPlan plan = row_plan(*a, dtype);
     CrossArgs p = cross_args(*a, dtype);
     p.out = out, p.lse = lse, p.rest = dtype == SVTAD_F32 ? nullptr : rest;
     p.splits = plan.splits, p.part = (float*)workspace;
@@ -140,15 +163,15 @@ extern "C" int svtad_cross_attention(const svtad_cross_args* a, void* out, float
 }
 
 template <typename T>
-static void cross_bwd(CrossArgs p, const svtad_cross_args& a, hipStream_t st) {
-    const RowPlan plan = row_plan(a);
+static void cross_bwd(CrossArgs p, const svtad_cross_args& a, int dtype, hipStream_t st) {
+    const RowPlan plan = row_plan(a, dtype);
     float* const part = p.part;
     if (p.M > 0) {
         p.splits = p.out ? plan.splits : 1;
         cross_bwd_q<T>(p, plan.wave_rows, st);
     }
     if (p.dk && a.nk > 0) {
-        p.splits = key_plan(a), p.part = part;
+        p.splits = key_plan(a, dtype), p.part = part;
         cross_bwd_kv<T>(p, st);
     }
 }
@@ -162,7 +185,7 @@ extern "C" int svtad_cross_attention_bwd(const svtad_cross_args* a, const void* 
     if ((!dq && !dk) || a->batch == 0) return SVTAD_OK;
     if (a->nq > 0 && (!a->q || !out || !lse || !dout || !dout_stride || (a->nk > 0 && (!a->k || !a->v))))
         return set_error(SVTAD_ERR_INVALID, "cross_attention_bwd: NULL pointer");
-    const size_t need = bwd_bytes(*a);
+    const size_t need = bwd_bytes(*a, dtype);
     if (need && (!workspace || workspace_bytes < need))
         return set_error(SVTAD_ERR_WORKSPACE, "cross_attention_bwd: workspace too small");
     CrossArgs p = cross_args(*a, dtype);
@@ -178,8 +201,8 @@ extern "C" int svtad_cross_attention_bwd(const svtad_cross_args* a, const void* 
     p.delta = (float*)workspace;
     p.part = (float*)((char*)workspace + align256((size_t)all_rows(*a) * 4));
     hipStream_t hs = (hipStream_t)stream;
-    if (dtype == SVTAD_F16) cross_bwd<f16>(p, *a, hs);
-    else if (dtype == SVTAD_BF16) cross_bwd<bf16>(p, *a, hs);
-    else cross_bwd<float>(p, *a, hs);
+    if (dtype == SVTAD_F16) cross_bwd<f16>(p, *a, dtype, hs);
+    else if (dtype == SVTAD_BF16) cross_bwd<bf16>(p, *a, dtype, hs);
+    else cross_bwd<float>(p, *a, dtype, hs);
     return launch_status();
 }

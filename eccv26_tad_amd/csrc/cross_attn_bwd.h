@@ -289,32 +289,30 @@ __global__ __launch_bounds__(256, (kResidentBwd<T, DP>)) void k_cross_bwd_kv(Cro
 }
 
 // The splits of dq added in order
-template <typename T>
+template <typename T, int G>
 __global__ __launch_bounds__(256) void k_cross_sum_q(CrossArgs p) {
-    const int dp = (p.D + 3) & ~3, nd = dp / 4, chunk = threadIdx.x & 63, g = threadIdx.x >> 6;
-    const int64_t rows = (int64_t)p.B * p.KH * p.M, e = (int64_t)blockIdx.x * 64 + chunk;
-    const bool in = e < rows * nd;
-    const f32x4 acc = join_groups(split_sum(p.part + (in ? e : 0) * 4, rows * dp, p.splits, g), g, chunk);
-    if (g != 0 || !in) return;
-    const int64_t at = e / nd, bh = at / p.M, r = at - bh * p.M, b = bh / p.KH;
-    const int j = (int)(bh - b * p.KH), c = (int)(e - at * nd) * 4;
-    store4<T>((T*)p.out + b * p.Nq * p.H * p.D + row_at(p, r, (int64_t)p.H * p.D, p.D, j), c, p.D, acc * p.scale);
+    const JoinChunk<G> j;
+    const uint32_t nd = (p.D + 3) / 4, rows = (uint32_t)(p.B * p.KH * p.M);
+    const bool in = j.e < rows * nd;
+    const f32x4 acc = join_groups<G>(split_sum<G>(p.part + (in ? (int64_t)j.e * 4 : 0), (int64_t)rows * nd * 4, p.splits, j.g), j);
+    if (j.g != 0 || !in) return;
+    const uint32_t at = j.e / nd, bh = at / (uint32_t)p.M, r = at - bh * (uint32_t)p.M, b = bh / p.KH, head = bh - b * p.KH;
+    store4<T>((T*)p.out + b * p.Nq * p.H * p.D + row_at(p, r, (int64_t)p.H * p.D, p.D, head), (int)(j.e - at * nd) * 4, p.D,
+              acc * p.scale);
 }
 
 // The splits of dk and dv
-template <typename T>
+template <typename T, int G>
 __global__ __launch_bounds__(256) void k_cross_sum_kv(CrossArgs p) {
-    const int dp = (p.D + 3) & ~3, nd = dp / 4, chunk = threadIdx.x & 63, g = threadIdx.x >> 6;
-    const int64_t rows = (int64_t)p.B * p.KH * p.Nk, all = rows * dp;
-    int64_t e = (int64_t)blockIdx.x * 64 + chunk;
-    const bool in = e < 2 * rows * nd, is_v = in && e >= rows * nd;
-    const f32x4 acc = join_groups(split_sum(p.part + (in ? e : 0) * 4, 2 * all, p.splits, g), g, chunk);
-    if (g != 0 || !in) return;
-    if (is_v) e -= rows * nd;
-    const int64_t at = e / nd, bh = at / p.Nk, n = at - bh * p.Nk, b = bh / p.KH;
-    const int j = (int)(bh - b * p.KH), c = (int)(e - at * nd) * 4;
-    T* const to = (T*)(is_v ? p.dv : p.dk) + ((b * p.Nk + n) * p.KH + j) * p.D;
-    store4<T>(to, c, p.D, is_v ? acc : acc * p.scale);
+    const JoinChunk<G> j;
+    const uint32_t nd = (p.D + 3) / 4, rows = (uint32_t)(p.B * p.KH * p.Nk), all = rows * nd;
+    const bool in = j.e < 2 * all, is_v = in && j.e >= all;
+    const f32x4 acc = join_groups<G>(split_sum<G>(p.part + (in ? (int64_t)j.e * 4 : 0), 2 * (int64_t)all * 4, p.splits, j.g), j);
+    if (j.g != 0 || !in) return;
+    const uint32_t e = is_v ? j.e - all : j.e, at = e / nd, bh = at / (uint32_t)p.Nk, n = at - bh * (uint32_t)p.Nk;
+    const uint32_t b = bh / p.KH, head = bh - b * p.KH;
+    T* const to = (T*)(is_v ? p.dv : p.dk) + ((b * p.Nk + n) * p.KH + head) * p.D;
+    store4<T>(to, (int)(e - at * nd) * 4, p.D, is_v ? acc : acc * p.scale);
 }
 
 template <typename T, int WM, int S>
@@ -335,7 +333,8 @@ void cross_bwd_q(const CrossArgs& p, int wave_rows, hipStream_t st) {
     else launch_cross_bwd_q<T, 1, 16>(p, st);
     if (p.splits > 1 && p.out) {
         const int64_t n = (int64_t)p.B * p.KH * p.M * ((p.D + 3) / 4);
-        k_cross_sum_q<T><<<(unsigned)cdiv(n, 64), 256, 0, st>>>(p);
+        if (p.splits <= kOneGroup) k_cross_sum_q<T, 1><<<(unsigned)cdiv(n, 256), 256, 0, st>>>(p);
+        else k_cross_sum_q<T, kJoinGroups><<<(unsigned)cdiv(n, 256 / kJoinGroups), 256, 0, st>>>(p);
     }
 }
 
@@ -350,7 +349,8 @@ void cross_bwd_kv(const CrossArgs& p, hipStream_t st) {
     else k_cross_bwd_kv<T, 128, true><<<grid, 256, 0, st>>>(p);
     if (p.splits > 1) {
         const int64_t n = 2 * (int64_t)p.B * p.KH * p.Nk * ((p.D + 3) / 4);
-        k_cross_sum_kv<T><<<(unsigned)cdiv(n, 64), 256, 0, st>>>(p);
+        if (p.splits <= kOneGroup) k_cross_sum_kv<T, 1><<<(unsigned)cdiv(n, 256), 256, 0, st>>>(p);
+        else k_cross_sum_kv<T, kJoinGroups><<<(unsigned)cdiv(n, 256 / kJoinGroups), 256, 0, st>>>(p);
     }
 }
 

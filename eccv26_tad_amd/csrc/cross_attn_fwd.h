@@ -291,34 +291,35 @@ __global__ __launch_bounds__(256, (kResidentFwd<T, DP>)) void k_cross_fwd(CrossA
 
 // The splits of a row joined in order, a chunk of 4 output values per thread of
 // each group
-template <typename T>
+template <typename T, int G>
 __global__ __launch_bounds__(256) void k_cross_join(CrossArgs p) {
-    __shared__ float red[kJoinGroups][64][2];
-    const int dp = (p.D + 3) & ~3, nd = dp / 4, chunk = threadIdx.x & 63, g = threadIdx.x >> 6;
-    const int64_t rows = (int64_t)p.B * p.KH * p.M, e = (int64_t)blockIdx.x * 64 + chunk;
-    const bool in = e < rows * nd;
-    const int64_t at = in ? e / nd : 0;
-    const int c = in ? (int)(e - at * nd) * 4 : 0;
-    const int per = (p.splits + kJoinGroups - 1) / kJoinGroups, s0 = lesser(p.splits, g * per), s1 = lesser(p.splits, s0 + per);
-    const float* const pm = p.part + (int64_t)p.splits * rows * dp + at * 2;
-    const float* const po = p.part + at * dp + c;
-    constexpr int kMost = 64 / kJoinGroups;  // splits of a group
+    __shared__ float red[G][256 / G][2];
+    const JoinChunk<G> j;
+    const uint32_t nd = (p.D + 3) / 4, rows = (uint32_t)(p.B * p.KH * p.M), at = j.e < rows * nd ? j.e / nd : 0;
+    const bool in = j.e < rows * nd;
+    const int dp = nd * 4, c = in ? (int)(j.e - at * nd) * 4 : 0;
+    const int per = (p.splits + G - 1) / G, s0 = lesser(p.splits, j.g * per), s1 = lesser(p.splits, s0 + per);
+    const float* const pm = p.part + ((int64_t)p.splits * rows * dp + (int64_t)at * 2);
+    const float* const po = p.part + ((int64_t)at * dp + c);
+    constexpr int kMost = G == 1 ? kOneGroup : kMaxSplits / G;  // splits of a group
     float m[kMost], w[kMost], top = kNegInf, l = 0.f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f}, v[kMost];
 #pragma unroll
     for (int i = 0; i < kMost; ++i)
         if (s0 + i < s1) {  // uniform
-            m[i] = pm[(s0 + i) * rows * 2];
-            w[i] = pm[(s0 + i) * rows * 2 + 1];
-            v[i] = *(const f32x4*)(po + (s0 + i) * rows * dp);
+            m[i] = pm[(int64_t)(s0 + i) * rows * 2];
+            w[i] = pm[(int64_t)(s0 + i) * rows * 2 + 1];
+            v[i] = *(const f32x4*)(po + (int64_t)(s0 + i) * rows * dp);
         }
 #pragma unroll
     for (int i = 0; i < kMost; ++i)
         if (s0 + i < s1) top = fmaxf(top, m[i]);
-    red[g][chunk][0] = top;
-    __syncthreads();
+    if constexpr (G > 1) {
+        red[j.g][j.chunk][0] = top;
+        __syncthreads();
 #pragma unroll
-    for (int q = 0; q < kJoinGroups; ++q) top = fmaxf(top, red[q][chunk][0]);
+        for (int q = 0; q < G; ++q) top = fmaxf(top, red[q][j.chunk][0]);
+    }
     if (top != kNegInf) {
 #pragma unroll
         for (int i = 0; i < kMost; ++i)
@@ -328,14 +329,13 @@ __global__ __launch_bounds__(256) void k_cross_join(CrossArgs p) {
                 acc += v[i] * f;
             }
     }
-    red[g][chunk][1] = l;
-    acc = join_groups(acc, g, chunk);  // its barrier covers red
-    if (g != 0 || !in) return;
+    if constexpr (G > 1) red[j.g][j.chunk][1] = l;
+    acc = join_groups<G>(acc, j);  // its barrier covers red
+    if (j.g != 0 || !in) return;
 #pragma unroll
-    for (int q = 1; q < kJoinGroups; ++q) l += red[q][chunk][1];
-    const int64_t bh = at / p.M, r = at - bh * p.M, b = bh / p.KH;
-    const int j = (int)(bh - b * p.KH);
-    const int64_t o = b * p.Nq * p.H * p.D + row_at(p, r, (int64_t)p.H * p.D, p.D, j);
+    for (int q = 1; q < G; ++q) l += red[q][j.chunk][1];
+    const uint32_t bh = at / (uint32_t)p.M, r = at - bh * (uint32_t)p.M, b = bh / p.KH, head = bh - b * p.KH;
+    const int64_t o = b * p.Nq * p.H * p.D + row_at(p, r, (int64_t)p.H * p.D, p.D, head);
     store4_rest<T>((T*)p.out + o, p.rest ? (T*)p.rest + o : nullptr, c, p.D, acc * (l == 0.f ? 0.f : 1.f / l));
     if (p.lse && c == 0) p.lse[at] = l == 0.f ? -kNegInf : top * p.c + __builtin_amdgcn_logf(l);
 }
@@ -358,7 +358,8 @@ void cross_fwd(const CrossArgs& p, int wave_rows, hipStream_t st) {
     else launch_cross_fwd<T, 1, 16>(p, st);
     if (p.splits > 1) {
         const int64_t n = (int64_t)p.B * p.KH * p.M * ((p.D + 3) / 4);
-        k_cross_join<T><<<(unsigned)cdiv(n, 64), 256, 0, st>>>(p);
+        if (p.splits <= kOneGroup) k_cross_join<T, 1><<<(unsigned)cdiv(n, 256), 256, 0, st>>>(p);
+        else k_cross_join<T, kJoinGroups><<<(unsigned)cdiv(n, 256 / kJoinGroups), 256, 0, st>>>(p);
     }
 }
 

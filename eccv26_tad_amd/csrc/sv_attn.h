@@ -349,20 +349,36 @@ __device__ __forceinline__ int64_t seen_length(const CrossArgs& p, int b) {
     return n < 0 ? 0 : n > p.Nk ? p.Nk : n;
 }
 
-// Splits are joined by workgroups of 64 chunks of 4 values by 4 thread groups,
-// each of which takes consecutive splits; the groups' sums are added in order.
-constexpr int kJoinGroups = 4;
-__device__ __forceinline__ f32x4 join_groups(f32x4 v, int g, int chunk) {
-    __shared__ f32x4 red[kJoinGroups - 1][64];
-    if (g > 0) red[g - 1][chunk] = v;
-    __syncthreads();
+// Splits are joined by workgroups of 256 / G chunks of 4 values by G thread
+// groups, each of which takes consecutive splits; the groups' sums are added in
+// order. Few splits take one group, whose loads are all in flight at once. No more
+// than 1024 workgroups write partial results, so that all chunks together are far
+// from 2^31: their divisions are 32 bits (24000 rows of 64 in two splits, the
+// forward with its join: 23.8 us so, 30.7 by four groups and with 64 bits).
+constexpr int kJoinGroups = 4, kOneGroup = 8, kMaxSplits = 64;  // groups, the most splits that one takes, and all take
+template <int G>
+struct JoinChunk {
+    static constexpr int kChunks = 256 / G;
+    uint32_t e;  // of all chunks
+    int chunk, g;
+    __device__ __forceinline__ JoinChunk() : e(blockIdx.x * kChunks + threadIdx.x % kChunks), chunk(threadIdx.x % kChunks), g(threadIdx.x / kChunks) {}
+};
+template <int G>
+__device__ __forceinline__ f32x4 join_groups(f32x4 v, const JoinChunk<G>& j) {
+    if constexpr (G == 1) return v;
+    else {
+        __shared__ f32x4 red[G - 1][JoinChunk<G>::kChunks];
+        if (j.g > 0) red[j.g - 1][j.chunk] = v;
+        __syncthreads();
 #pragma unroll
-    for (int q = 1; q < kJoinGroups; ++q) v += red[q - 1][chunk];
-    return v;
+        for (int q = 1; q < G; ++q) v += red[q - 1][j.chunk];
+        return v;
+    }
 }
 // This thread's share of a chunk's splits, `stride` floats apart, from p on
+template <int G>
 __device__ __forceinline__ f32x4 split_sum(const float* p, int64_t stride, int splits, int g) {
-    const int per = (splits + kJoinGroups - 1) / kJoinGroups, s0 = lesser(splits, g * per), n = lesser(splits, s0 + per) - s0;
+    const int per = (splits + G - 1) / G, s0 = lesser(splits, g * per), n = lesser(splits, s0 + per) - s0;
     float a[4] = {0.f, 0.f, 0.f, 0.f};
     add_strided(a, p + s0 * stride, stride, n);
     return f32x4{a[0], a[1], a[2], a[3]};

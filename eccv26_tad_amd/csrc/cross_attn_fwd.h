@@ -11,7 +11,10 @@
 // workgroups, whose partial sums k_cross_join adds in a fixed order.
 //
 // Probabilities are rounded to T for the product with v (the matrix units'
-// operand type); their sum, the scale and the output's sums stay float32.
+// operand type); their sum, the scale and the output's sums stay float32. Over the
+// keys of a lone tile a second product adds what that rounding took: the backward's
+// delta is made from the output, and with few keys its error would reach the
+// gradients unaveraged.
 // Keys that are not seen are staged as zeros and their scores replaced, so
 // neither infinities nor NaN in their places reach a result.
 #pragma once
@@ -58,7 +61,8 @@ struct KeyTiles {
           mask(p.mask ? p.mask + b * p.mask_b : nullptr), len(seen_length(p, b)), mem(mem), start_mem(start_mem) {
         const uint32_t tiles = (uint32_t)cdiv(len, TK), per = (tiles + p.splits - 1) / p.splits;
         t0 = split * per, t1 = lesser(tiles, split * per + per);
-        tw = mask ? t0 : max<int64_t>(t0, lesser<int64_t>(t1, len / TK));
+        // a tile alone goes the way of those with unseen keys
+        tw = mask || tiles < 2 ? t0 : max<int64_t>(t0, lesser<int64_t>(t1, len / TK));
     }
 
     __device__ __forceinline__ int left(int64_t tile) const { return (int)lesser<int64_t>(len - tile * TK, TK); }
@@ -174,6 +178,15 @@ __global__ __launch_bounds__(256, (kResidentFwd<T, DP>)) void k_cross_fwd(CrossA
     float m = kNegInf, l = 0.f;
 #pragma unroll
     for (int db = 0; db < DB; ++db) acc[db] = M::fill(0.f);
+    auto values = [&](const unsigned char* lv, const Acc* s) __attribute__((always_inline)) {
+#pragma unroll
+        for (int kk = 0; kk < KW / M::K; ++kk) {
+            const Frag8<T> pf = M::pack(s, kk);
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+                acc[db] = M::mma(M::template frag_t<W>(lv, wk * KW + kk * M::K, db, lane), pf, acc[db]);
+        }
+    };
     auto use = [&](int64_t tile, auto part) __attribute__((always_inline)) {
         const unsigned char *const lk = keys.keys(tile), *const lv = keys.values(tile);
         Acc s[NB];
@@ -206,13 +219,15 @@ __global__ __launch_bounds__(256, (kResidentFwd<T, DP>)) void k_cross_fwd(CrossA
                 s[nb][e] = __builtin_amdgcn_exp2f(fmaf(s[nb][e], p.c, -mc));
                 l += s[nb][e];
             }
+        values(lv, s);
+        if constexpr (part.value && sizeof(T) == 2)
+            if (keys.len <= TK) {
 #pragma unroll
-        for (int kk = 0; kk < KW / M::K; ++kk) {
-            const Frag8<T> pf = M::pack(s, kk);
+                for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-            for (int db = 0; db < DB; ++db)
-                acc[db] = M::mma(M::template frag_t<W>(lv, wk * KW + kk * M::K, db, lane), pf, acc[db]);
-        }
+                    for (int e = 0; e < 4 * M::Q; ++e) s[nb][e] -= (float)(T)s[nb][e];
+                values(lv, s);
+            }
     };
     keys.walk(p, [&](int64_t t) { use(t, std::false_type()); }, [&](int64_t t) { use(t, std::true_type()); });
     l = M::col_sum(l);

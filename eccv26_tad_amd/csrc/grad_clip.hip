@@ -14,7 +14,9 @@
 // Squares are summed in float64: float32 gradients neither overflow nor lose
 // small addends, at a rate the vector units outrun memory at (bound by its
 // bytes). Every workgroup leaves one partial sum; the scaling pass adds them
-// in one fixed order in each of its workgroups, without a launch between.
+// in one fixed order in each of its workgroups, without a launch between. Both
+// are bound by memory (326 M elements of bfloat16 into float32: the norm 132 us, 4.9
+// TB/s, the scaling 428 us, 4.6 TB/s).
 #include <algorithm>
 #include <type_traits>
 
@@ -194,7 +196,9 @@ __global__ __launch_bounds__(256) void k_grad_scale(ClipList t, ClipScale s) {
 }
 
 // Workgroups for `total` elements: one for every 16 KB or so, at most four per
-// compute unit in the norm's pass (each leaves a partial sum), eight in the other.
+// compute unit in the norm's pass (each leaves a partial sum), eight in the other
+// (25 tensors of 16 K in bfloat16 8.0 us, 8.6 with one for 64 KB; 25 of 256 K 15.9,
+// 17.1 with half as many in the scaling pass).
 static int clip_groups(int64_t total, int most = kMaxGroups) {
     return (int)std::max<int64_t>(1, std::min<int64_t>(cdiv(total, 4096), most));
 }

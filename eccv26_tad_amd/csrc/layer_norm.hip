@@ -6,7 +6,8 @@
 //   dw = sum over rows of dy xhat,  db = sum over rows of dy
 //
 // A row stays in registers between its sums and its store, so memory sees it
-// once; the kernels are bound by its bytes. A group of G lanes holds a row, K
+// once; the kernels are bound by its bytes (49154 x 1024 in bfloat16: forward 33 us,
+// 6.0 TB/s, backward 56 us, 5.4 TB/s; a copy reaches 5.2 to 5.6). A group of G lanes holds a row, K
 // vectors of 16 bytes per lane (lane g's vector j starts at (j G + g) V): G is
 // the power of two up to 64 that covers the width with one vector, so that the
 // short rows of per-head norms share a wave, and beyond a wave's 4 vectors per
@@ -301,7 +302,10 @@ __global__ __launch_bounds__(256) void k_layer_norm_sum(const float* __restrict_
 
 // Lanes of a row's group and vectors per lane: the smallest power of two of
 // lanes that takes the row at one vector each, at most a wave; then up to 4
-// vectors per lane; then a workgroup per row (0 lanes).
+// vectors per lane; then a workgroup per row (0 lanes). A wave per row against a
+// workgroup, forward and backward: 49154 x 1024 in bfloat16 32 + 58 us against 92 +
+// 337, 20000 x 2048 33 + 56 against 44 + 139, 20000 x 1024 in float32 27 + 45
+// against 27 + 58. Beyond 4 vectors a wave's registers do not hold the row twice.
 struct LnShape {
     int lanes, k;
     bool tail;
@@ -317,7 +321,8 @@ static LnShape ln_shape(int c, int dtype) {
 }
 
 // Workgroups of the backward: as many as the 256 compute units hold at two
-// each, and no more than the rows need.
+// each, and no more than the rows need (49154 x 1024 in bfloat16: 58 us with 512, 89
+// with 256, 66 with 1024, whose partial sums cost more).
 static int ln_bwd_groups(int64_t rows, const LnShape& s) {
     const int per = s.lanes ? 256 / s.lanes : 1;
     return (int)std::max<int64_t>(1, std::min<int64_t>(cdiv(rows, per), 512));

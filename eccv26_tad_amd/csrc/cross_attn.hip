@@ -11,18 +11,19 @@ constexpr int kMaxHeadDim = 128;
 // Splits of an axis of `tiles` tiles for `groups` workgroups of `rows` results:
 // as many as fill one, two, three or four workgroups per compute unit, or none,
 // whichever is estimated to take least. The estimate is in times of one tile on a
-// compute unit of its own, 0.87 us in bfloat16 at a head dimension of 64. Two and
-// more workgroups share a unit and take 0.75 of it each, unless one fills it:
-// float32 and wide heads, whose tiles take twice as long as well. Partial results
-// cost a launch (5) and their writing, reading and adding (0.03 for 128 rows of
-// 64). Measured there, 1000 rows, forward, split against whole: 48 groups over 1500
+// compute unit of its own: for two products 0.87 us in 16 bits at a head dimension
+// of 64, 7 times as much in float32. Two and more workgroups share a unit and take 0.75 of it each,
+// unless one fills it (float32, wide heads). Partial results cost a launch (4.4 us)
+// and their writing, reading and adding (0.026 us for 128 rows of 64). Measured in
+// bfloat16 at 64, 1000 rows, forward, split against whole: 48 groups over 1500
 // keys 17.5 us in four against 25.9, 192 over 500 keys 23.8 in two against 12.3, 192
 // over 20000 keys 176 in four against 202 in two and 277. One query over 8 x 31361
-// keys of 4 heads: 47.3 us in 16, 53.5 in 8, 55.1 in 24. Of 222 kernels at 74 drawn
-// sizes of all types 6 took over 15 % more than in the best of 14 splits (34 % most).
-static int splits(const svtad_cross_args& a, int dtype, int64_t groups, int64_t tiles, int rows) {
+// keys of 4 heads: 47.3 us in 16, 53.5 in 8, 55.1 in 24. Of 285 kernels at 95 drawn
+// sizes of all types 7 took over 15 % more than in the best of 14 splits (27 % most).
+static int splits(const svtad_cross_args& a, int dtype, int64_t groups, int64_t tiles, int rows, double products) {
     const bool alone = dtype == SVTAD_F32 || a.head_dim > 64;
-    const double launch = alone ? 2.5 : 5, part = (alone ? 0.015 : 0.03) * rows * a.head_dim / (128 * 64);
+    const double tile = products / 2. * (dtype == SVTAD_F32 ? 7 : 1) * (0.5 + a.head_dim / 128.);
+    const double launch = 5 / tile, part = 0.03 * rows * a.head_dim / (128 * 64) / tile;
     int best = 1;
     double least = (double)tiles * (double)cdiv(groups, 256);
     for (int rounds = 1; rounds <= 4 && groups > 0; ++rounds) {
@@ -48,14 +49,14 @@ static RowPlan row_plan(const svtad_cross_args& a, int dtype) {
     const int64_t m = a.nq * (a.heads / a.kv_heads);
     RowPlan r{m <= 16 ? 1 : m <= 64 ? 2 : 4, 1};
     const int rows = r.wave_rows == 4 ? 128 : r.wave_rows == 2 ? 64 : 16;
-    r.splits = splits(a, dtype, cdiv(m, rows) * a.batch * a.kv_heads, cdiv(a.nk, r.wave_rows == 1 ? 128 : 64), rows);
+    r.splits = splits(a, dtype, cdiv(m, rows) * a.batch * a.kv_heads, cdiv(a.nk, r.wave_rows == 1 ? 128 : 64), rows, 2);
     return r;
 }
 
 // Splits of the rows in the kernel over key tiles.
 static int key_plan(const svtad_cross_args& a, int dtype) {
     const int64_t m = a.nq * (a.heads / a.kv_heads);
-    return splits(a, dtype, cdiv(a.nk, kCrossKvKeys) * a.batch * a.kv_heads, cdiv(m, 64), kCrossKvKeys);
+    return splits(a, dtype, cdiv(a.nk, kCrossKvKeys) * a.batch * a.kv_heads, cdiv(m, 64), kCrossKvKeys, 3.4);  // four, and what they share
 }
 
 static size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }

@@ -6,12 +6,13 @@
 //   dw = sum over rows of dy xhat,  db = sum over rows of dy
 //
 // A row stays in registers between its sums and its store, so memory sees it
-// once; the kernels are bound by its bytes (49154 x 1024 in bfloat16: forward 33 us,
-// 6.0 TB/s, backward 56 us, 5.4 TB/s; a copy reaches 5.2 to 5.6). A group of G lanes holds a row, K
-// vectors of 16 bytes per lane (lane g's vector j starts at (j G + g) V): G is
-// the power of two up to 64 that covers the width with one vector, so that the
-// short rows of per-head norms share a wave, and beyond a wave's 4 vectors per
-// lane a whole workgroup takes a row. Sums and statistics are float32.
+// once; the kernels are bound by its bytes (49154 x 1024 in bfloat16: forward 33
+// us, 6.0 TB/s, backward 56 us, 5.4 TB/s; a copy reaches 5.2 to 5.6). A group of G
+// lanes holds a row, K vectors of 16 bytes per lane (lane g's vector j starts at
+// (j G + g) V): G is the power of two up to 64 that covers the width with one
+// vector, so that the short rows of per-head norms share a wave, and beyond a
+// wave's 3 or 4 vectors per lane a whole workgroup takes a row. Sums and
+// statistics are float32.
 #include <algorithm>
 
 #include "sv_internal.h"
@@ -90,12 +91,13 @@ __device__ __forceinline__ void load_params(float (&f)[kVec<T>], const void* p, 
     }
 }
 
-// Sums over a row's lanes; WG: the workgroup's 4 waves hold one row.
+// Sums over a row's lanes; WG: the workgroup's 4 waves hold one row and meet in
+// red. The next sum goes through another red, the one after through this again: by
+// then all have passed that one's barrier.
 template <bool WG>
 __device__ __forceinline__ float row_sum(float v, int lanes, float* red) {
     v = group_sum(v, lanes);
     if constexpr (WG) {
-        __syncthreads();  // red's last readers are done
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
         __syncthreads();
         v = (red[0] + red[1]) + (red[2] + red[3]);
@@ -106,7 +108,7 @@ __device__ __forceinline__ float row_sum(float v, int lanes, float* red) {
 template <typename T, int K, bool WG, bool TAIL>
 __global__ __launch_bounds__(256) void k_layer_norm(LnArgs p) {
     constexpr int V = kVec<T>;
-    __shared__ float red[4];
+    __shared__ float red[2][4];
     const int G = WG ? 256 : p.lanes, g = threadIdx.x & (G - 1), per = 256 / G, c = p.c;
     float w[K][V], b[K][V];
 #pragma unroll
@@ -126,7 +128,7 @@ __global__ __launch_bounds__(256) void k_layer_norm(LnArgs p) {
 #pragma unroll
             for (int e = 0; e < V; ++e) s += f[j][e];
         }
-        const float mean = row_sum<WG>(s, min(G, 64), red) * ic;
+        const float mean = row_sum<WG>(s, min(G, 64), red[0]) * ic;
         s = 0.f;
 #pragma unroll
         for (int j = 0; j < K; ++j) {
@@ -137,7 +139,7 @@ __global__ __launch_bounds__(256) void k_layer_norm(LnArgs p) {
                 if (TAIL ? c0 + e < c : c0 < c) s += f[j][e] * f[j][e];
             }
         }
-        const float rstd = rsqrtf(row_sum<WG>(s, min(G, 64), red) * ic + p.eps);
+        const float rstd = rsqrtf(row_sum<WG>(s, min(G, 64), red[1]) * ic + p.eps);
         if (!in) continue;
         T* const y = (T*)p.y + r * c;
 #pragma unroll
@@ -189,7 +191,7 @@ struct LnRow {
 template <typename T, int K, bool WG, bool TAIL>
 __global__ __launch_bounds__(256) void k_layer_norm_bwd(LnArgs p) {
     constexpr int V = kVec<T>, W = 64 * K * V;  // the widest row of a wave's group
-    __shared__ float red[4];
+    __shared__ float red[2][2][4];  // [row's parity]
     const int G = WG ? 256 : p.lanes, g = threadIdx.x & (G - 1), per = 256 / G, c = p.c;
     float w[K][V], sw[K][V], sb[K][V];
 #pragma unroll
@@ -199,6 +201,7 @@ __global__ __launch_bounds__(256) void k_layer_norm_bwd(LnArgs p) {
         for (int e = 0; e < V; ++e) sw[j][e] = sb[j][e] = 0.f;
     }
     const float ic = 1.f / c;
+    int odd = 0;
     const int64_t step = (int64_t)gridDim.x * per;
     LnRow<T, K, TAIL> next;
     next.load(p, (int64_t)blockIdx.x * per + threadIdx.x / G, G, g);
@@ -221,8 +224,15 @@ __global__ __launch_bounds__(256) void k_layer_norm_bwd(LnArgs p) {
             }
         }
         if (!p.y) continue;
-        s1 = row_sum<WG>(s1, min(G, 64), red) * ic;
-        s2 = row_sum<WG>(s2, min(G, 64), red) * ic;
+        s1 = group_sum(s1, min(G, 64)), s2 = group_sum(s2, min(G, 64));
+        if constexpr (WG) {  // both through one barrier
+            if ((threadIdx.x & 63) == 0) red[odd][0][threadIdx.x >> 6] = s1, red[odd][1][threadIdx.x >> 6] = s2;
+            __syncthreads();
+            s1 = (red[odd][0][0] + red[odd][0][1]) + (red[odd][0][2] + red[odd][0][3]);
+            s2 = (red[odd][1][0] + red[odd][1][1]) + (red[odd][1][2] + red[odd][1][3]);
+            odd ^= 1;
+        }
+        s1 *= ic, s2 *= ic;
         if (!row.in) continue;
         T* const dx = (T*)p.y + r * c;
 #pragma unroll
@@ -302,30 +312,32 @@ __global__ __launch_bounds__(256) void k_layer_norm_sum(const float* __restrict_
 
 // Lanes of a row's group and vectors per lane: the smallest power of two of
 // lanes that takes the row at one vector each, at most a wave; then up to 4
-// vectors per lane; then a workgroup per row (0 lanes). A wave per row against a
-// workgroup, forward and backward: 49154 x 1024 in bfloat16 32 + 58 us against 92 +
-// 337, 20000 x 2048 33 + 56 against 44 + 139, 20000 x 1024 in float32 27 + 45
-// against 27 + 58. Beyond 4 vectors a wave's registers do not hold the row twice.
+// vectors per lane (3 in the forward); then a workgroup per row (0 lanes). A wave
+// per row against a workgroup, forward and backward: 49154 x 1024 in bfloat16 32 +
+// 58 us against 51 + 150, 20000 x 1536 23 + 37 against 25 + 58, 20000 x 2048 33 + 55
+// against 28 + 61, 20000 x 1024 in float32 28 + 44 against 26 + 48.
 struct LnShape {
     int lanes, k;
     bool tail;
 };
 
-static LnShape ln_shape(int c, int dtype) {
+static LnShape ln_shape(int c, int dtype, bool bwd) {
     const int v = dtype == SVTAD_F32 ? 4 : 8, vecs = (int)cdiv(c, v);
     LnShape s{1, 1, c % v != 0};
     while (s.lanes < vecs && s.lanes < 64) s.lanes *= 2;
     if (vecs > 64) s.k = (int)cdiv(vecs, 64);
-    if (s.k > 4) s.lanes = 0, s.k = (int)cdiv(vecs, 256) <= 4 ? 4 : 8;
+    if (s.k > (bwd ? 4 : 3)) s.lanes = 0, s.k = vecs <= 512 ? 2 : vecs <= 1024 ? 4 : 8;
     return s;
 }
 
 // Workgroups of the backward: as many as the 256 compute units hold at two
-// each, and no more than the rows need (49154 x 1024 in bfloat16: 58 us with 512, 89
-// with 256, 66 with 1024, whose partial sums cost more).
-static int ln_bwd_groups(int64_t rows, const LnShape& s) {
+// each, and no more than the rows need (49154 x 1024 in bfloat16: 58 us with 512, 88
+// with 256, 66 with 1024, whose partial sums cost more); one each for rows so wide
+// that partial sums weigh more still (5000 x 8192 in bfloat16 65 us against 78 with
+// 512, 10000 x 4096 63 against 54).
+static int ln_bwd_groups(int64_t rows, int c, const LnShape& s) {
     const int per = s.lanes ? 256 / s.lanes : 1;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(cdiv(rows, per), 512));
+    return (int)std::max<int64_t>(1, std::min<int64_t>(cdiv(rows, per), c > 4096 ? 256 : 512));
 }
 
 template <typename T, int K, bool WG>
@@ -333,7 +345,7 @@ static void launch_ln(const LnArgs& a, bool bwd, bool tail, int grid, hipStream_
     if (bwd) {
         if (tail) k_layer_norm_bwd<T, K, WG, true><<<grid, 256, 0, st>>>(a);
         else k_layer_norm_bwd<T, K, WG, false><<<grid, 256, 0, st>>>(a);
-    } else {
+    } else if constexpr (WG || K < 4) {
         if (tail) k_layer_norm<T, K, WG, true><<<grid, 256, 0, st>>>(a);
         else k_layer_norm<T, K, WG, false><<<grid, 256, 0, st>>>(a);
     }
@@ -345,6 +357,7 @@ static void launch_ln_type(const LnArgs& a, bool bwd, const LnShape& s, int grid
         if constexpr (sizeof(T) == 4) {
             if (s.k == 8) return launch_ln<T, 8, true>(a, bwd, s.tail, grid, st);
         }
+        if (s.k == 2) return launch_ln<T, 2, true>(a, bwd, s.tail, grid, st);
         return launch_ln<T, 4, true>(a, bwd, s.tail, grid, st);
     }
     switch (s.k) {
@@ -397,7 +410,7 @@ using namespace svtad;
 extern "C" int svtad_norm(const svtad_norm_args* p, void* y, int dtype, void* stream) {
     const int st = ln_check(p, dtype);
     if (st) return st;
-    const LnShape s = ln_shape(p->c, dtype);
+    const LnShape s = ln_shape(p->c, dtype, false);
     LnArgs a = ln_args(p, s);
     if (a.rows == 0) return SVTAD_OK;
     if (!p->x || !y) return set_error(SVTAD_ERR_INVALID, "layer_norm: NULL pointer");
@@ -409,21 +422,21 @@ extern "C" int svtad_norm(const svtad_norm_args* p, void* y, int dtype, void* st
 
 extern "C" size_t svtad_norm_bwd_workspace_bytes(int64_t rows, int c, int dtype) {
     if (rows < 1 || c < 1 || c > kMaxWidth) return 0;
-    return (size_t)ln_bwd_groups(rows, ln_shape(c, dtype)) * 2 * (size_t)c * sizeof(float);
+    return (size_t)ln_bwd_groups(rows, c, ln_shape(c, dtype, true)) * 2 * (size_t)c * sizeof(float);
 }
 
 extern "C" int svtad_norm_bwd(const svtad_norm_args* p, const void* dy, void* dx, void* dw, void* db, void* workspace,
                               size_t workspace_bytes, int dtype, void* stream) {
     const int st = ln_check(p, dtype);
     if (st) return st;
-    const LnShape s = ln_shape(p->c, dtype);
+    const LnShape s = ln_shape(p->c, dtype, true);
     LnArgs a = ln_args(p, s);
     const bool sums = dw || db;
     hipStream_t hs = (hipStream_t)stream;
     int grid = 0;
     if (a.rows > 0) {
         if (!p->x || !dy || !p->stats) return set_error(SVTAD_ERR_INVALID, "layer_norm_bwd: NULL pointer");
-        grid = ln_bwd_groups(a.rows, s);
+        grid = ln_bwd_groups(a.rows, a.c, s);
         if (sums && (!workspace || workspace_bytes < svtad_norm_bwd_workspace_bytes(a.rows, a.c, dtype)))
             return set_error(SVTAD_ERR_WORKSPACE, "layer_norm_bwd: workspace too small");
         a.dy = dy, a.y = dx, a.part = sums ? (float*)workspace : nullptr;

@@ -238,3 +238,24 @@ def test_refusals(dev):
         sv.layer_norm(x, w, eps=-1.0)
     with pytest.raises(RuntimeError, match="GPU tensor"):
         sv.layer_norm(x, w.cpu())
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("rows,c", [(1600, 1280), (1600, 2056), (1100, 5000), (900, 8192)])
+def test_several_wide_rows_per_workgroup(dev, rows, c, dtype):
+    """The rows of a workgroup follow one another in the backward; twice the same bits."""
+    import eccv26_tad_amd as sv
+
+    x = torch.randn(rows, c, device=dev).to(DTYPES[dtype]).requires_grad_(True)
+    w, b = torch.rand(c, device=dev).requires_grad_(True), torch.randn(c, device=dev).requires_grad_(True)
+    dy = torch.randn(rows, c, device=dev).to(DTYPES[dtype])
+    y = sv.layer_norm(x, w, b, 1e-6)
+    got = torch.autograd.grad(y, (x, w, b), dy)
+    again = torch.autograd.grad(sv.layer_norm(x, w, b, 1e-6), (x, w, b), dy)
+    X, W, B = (t.detach().double().requires_grad_(True) for t in (x, w, b))
+    Y = torch.nn.functional.layer_norm(X, (c,), W, B, 1e-6)
+    want = torch.autograd.grad(Y, (X, W, B), dy.double())
+    u = {"f16": 2.0 ** -11, "bf16": 2.0 ** -8, "f32": 2e-6}[dtype]  # y and dx are rounded once; dw and db are float32 sums
+    for a, e, tol in ((y, Y, u), (got[0], want[0], u), (got[1], want[1], 1e-5), (got[2], want[2], 1e-5)):
+        assert float((a.double() - e).norm() / e.norm()) <= tol
+    assert all(torch.equal(a, e) for a, e in zip(got, again))

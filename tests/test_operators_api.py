@@ -99,7 +99,6 @@ def test_cross_attention(lib):
         _cross(**kw), None, None, None, None, None, None, dk, dv, None, Z, F16, None)
     assert bwd(dk=P(16)) == INVALID and b"together" in lib.svtad_last_error()
     assert bwd() == OK and bwd(dk=P(16), dv=P(16)) == INVALID
-    assert bwd(dk=P(16), dv=P(16), nq=0) == WORKSPACE or bwd(dk=P(16), dv=P(16), nq=0) in (OK, 100)
 
 
 def test_grad_clip(lib):

@@ -243,30 +243,33 @@ __device__ __forceinline__ uint32_t lds_offset(const void* p) {
 // LDS the compiler waits for the loads to LDS that it knows of, as it cannot
 // tell which of two tiles they go to, and no load would be in flight during the
 // work on the tile before. There is no output register; `landed` waits. m0, which
-// holds the LDS address, is set in the same statement and holds nothing else here.
+// holds the LDS address, is set in the same statement. The compiler cannot see into
+// it either: a descriptor's words may come from a vector instruction
+// (v_readfirstlane) right before the statement, and a load may read them 5 wait
+// states later at the earliest. The write of m0 is one, the s_nop the other 4.
 // ONCE: memory that nobody reads again, not kept in the caches.
 template <bool ONCE>
 __device__ __forceinline__ void load_to_lds(u32x4 r, uint32_t offset, const unsigned char* to) {
     const uint32_t base = lds_offset(to);
     if constexpr (ONCE)
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds"
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds"
                      :
                      : "s"(base), "v"(offset), "s"(r)
-                     : "memory");
+                     : "memory", "m0");
     else
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                      :
                      : "s"(base), "v"(offset), "s"(r)
-                     : "memory");
+                     : "memory", "m0");
 }
 
 // The same for 4 bytes per lane.
 __device__ __forceinline__ void load_word_to_lds(u32x4 r, uint32_t offset, const void* to) {
     const uint32_t base = lds_offset(to);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dword %1, %2, 0 offen lds"
                  :
                  : "s"(base), "v"(offset), "s"(r)
-                 : "memory");
+                 : "memory", "m0");
 }
 
 // One thread's share of loading a tile of TILE rows by W elements to LDS through

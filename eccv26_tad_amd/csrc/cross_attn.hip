@@ -184,7 +184,9 @@ extern "C" int svtad_cross_attention_bwd(const svtad_cross_args* a, const void* 
     if (st) return st;
     if (!dk != !dv) return set_error(SVTAD_ERR_INVALID, "cross_attention_bwd: dk and dv come together");
     if ((!dq && !dk) || a->batch == 0) return SVTAD_OK;
-    if (a->nq > 0 && (!a->q || !out || !lse || !dout || !dout_stride || (a->nk > 0 && (!a->k || !a->v))))
+    // without queries dk and dv are written all the same, by a kernel that holds k and v
+    if ((a->nq > 0 && (!a->q || !out || !lse || !dout || !dout_stride)) ||
+        (a->nk > 0 && (a->nq > 0 || dk) && (!a->k || !a->v)))
         return set_error(SVTAD_ERR_INVALID, "cross_attention_bwd: NULL pointer");
     const size_t need = bwd_bytes(*a, dtype);
     if (need && (!workspace || workspace_bytes < need))

@@ -155,3 +155,14 @@ def test_module_parameters():
         "q_norm.weight": (16,), "q_norm.bias": (16,), "k_norm.weight": (16,), "k_norm.bias": (16,),
         "q.weight": (96, 96), "q.bias": (96,), "kv.weight": (64, 40), "kv.bias": (64,), "proj.weight": (96, 96),
         "proj.bias": (96,)}
+
+
+def test_cross_attention_bwd_without_queries(lib):
+    """dk and dv of no queries are zeros, which the kernel that holds k and v
+    writes: both have to be there, as with queries."""
+    Z = ctypes.c_size_t(0)
+    bwd = lambda **kw: lib.svtad_cross_attention_bwd(  # noqa: E731
+        _cross(nq=0, **kw), None, None, None, None, None, None, P(16), P(16), None, Z, F16, None)
+    for given in (dict(), dict(k=16), dict(v=16)):
+        assert bwd(**given) == INVALID and b"NULL" in lib.svtad_last_error()
+    assert bwd(batch=0) == OK

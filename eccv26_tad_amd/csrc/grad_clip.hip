@@ -18,6 +18,7 @@
 // are bound by memory (326 M elements of bfloat16 into float32: the norm 132 us, 4.9
 // TB/s, the scaling 428 us, 4.6 TB/s).
 #include <algorithm>
+#include <cstdlib>
 #include <type_traits>
 
 #include "sv_internal.h"
@@ -203,9 +204,71 @@ static int clip_groups(int64_t total, int most = kMaxGroups) {
     return (int)std::max<int64_t>(1, std::min<int64_t>(cdiv(total, 4096), most));
 }
 
+static int64_t type_size(int dtype) { return dtype == SVTAD_F16 || dtype == SVTAD_BF16 ? 2 : 4; }
+
+static bool share(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+    return (uintptr_t)a < (uintptr_t)b + b_bytes && (uintptr_t)b < (uintptr_t)a + a_bytes;
+}
+
+// How the memory of a list's tensors is shared. Workgroups of a launch run in no
+// order, so what one of them writes no other may read or write.
+enum class Shared {
+    kNo,
+    kRepeats,  // tensors written in place alone: in launches of their own each mention scales
+    kBad,      // an output and something else
+    kUnknown,  // no host memory to find out
+};
+
+// Tensors in the order of their addresses, outputs beside them or in place, are
+// seen to be apart in one walk; others are sorted.
+static Shared shared(const svtad_grad* t, int64_t count) {
+    enum { READ, OUT, IN_PLACE };
+    struct Span {
+        uintptr_t lo, hi;
+        int kind;
+    };
+    uintptr_t g_lo = UINTPTR_MAX, g_hi = 0, o_lo = UINTPTR_MAX, o_hi = 0;
+    bool ordered = true;
+    for (int64_t i = 0; i < count; ++i) {
+        if (t[i].count <= 0) continue;
+        const uintptr_t g = (uintptr_t)t[i].g, o = (uintptr_t)t[i].out;
+        ordered = ordered && g >= g_hi;
+        g_lo = std::min(g_lo, g), g_hi = std::max<uintptr_t>(g_hi, g + t[i].count * type_size(t[i].g_type));
+        if (o == g && t[i].g_type == t[i].out_type) continue;
+        ordered = ordered && o >= o_hi;
+        o_lo = std::min(o_lo, o), o_hi = std::max<uintptr_t>(o_hi, o + t[i].count * type_size(t[i].out_type));
+    }
+    if (ordered && (o_lo >= g_hi || g_lo >= o_hi)) return Shared::kNo;
+    Span* const spans = (Span*)malloc((size_t)count * 2 * sizeof(Span));
+    if (!spans) return Shared::kUnknown;
+    int64_t n = 0;
+    for (int64_t i = 0; i < count; ++i) {
+        if (t[i].count <= 0) continue;
+        const uintptr_t g = (uintptr_t)t[i].g, o = (uintptr_t)t[i].out;
+        const bool in_place = o == g && t[i].g_type == t[i].out_type;
+        spans[n++] = {g, g + t[i].count * type_size(t[i].g_type), in_place ? IN_PLACE : READ};
+        if (!in_place) spans[n++] = {o, o + t[i].count * type_size(t[i].out_type), OUT};
+    }
+    std::sort(spans, spans + n, [](const Span& a, const Span& b) { return a.lo < b.lo; });
+    Shared found = Shared::kNo;
+    uintptr_t hi[3] = {0, 0, 0};  // where those so far end, by kind
+    for (int64_t i = 0; i < n && found != Shared::kBad; ++i) {
+        const Span& s = spans[i];
+        for (int kind : {READ, OUT, IN_PLACE}) {
+            if (s.lo >= hi[kind] || (s.kind == READ && kind == READ)) continue;
+            if (s.kind != IN_PLACE || kind != IN_PLACE) found = Shared::kBad;
+            else if (found == Shared::kNo) found = Shared::kRepeats;
+        }
+        hi[s.kind] = std::max(hi[s.kind], s.hi);
+    }
+    free(spans);
+    return found;
+}
+
 struct ClipPlan {  // the launches of a list of tensors of any length
     const svtad_grad* t;
     int64_t count;
+    bool once = false;  // no memory twice in a launch: one that writes it
 
     // The tensors from `at` on that one launch takes: one pair of types, none
     // empty. Returns the next tensor's number.
@@ -217,6 +280,12 @@ struct ClipPlan {  // the launches of a list of tensors of any length
             if (q.count == 0) continue;
             if (l.count == 0) l.g_type = q.g_type, l.out_type = q.out_type;
             else if (l.g_type != q.g_type || l.out_type != q.out_type || (l.g[0] == l.out[0]) != (q.g == q.out)) break;
+            if (once) {
+                const int64_t size = type_size(q.g_type);
+                int i = 0;
+                while (i < l.count && !share(q.g, q.count * size, l.g[i], (l.end[i] - (i ? l.end[i - 1] : 0)) * size)) ++i;
+                if (i < l.count) break;
+            }
             l.g[l.count] = q.g, l.out[l.count] = q.out;
             total += q.count;
             l.end[l.count++] = total;
@@ -276,6 +345,9 @@ extern "C" int svtad_grad_clip(const svtad_grad* tensors, int64_t count, int nor
     if (norm_type != SVTAD_NORM_2 && norm_type != SVTAD_NORM_INF)
         return set_error(SVTAD_ERR_INVALID, "grad_clip: norm_type must be the 2-norm or the maximum");
     if (!norm) return set_error(SVTAD_ERR_INVALID, "grad_clip: NULL pointer");
+    const Shared memory = write ? shared(tensors, count) : Shared::kNo;
+    if (memory == Shared::kBad) return set_error(SVTAD_ERR_INVALID, "grad_clip: an output shares memory with another tensor");
+    if (memory == Shared::kUnknown) return set_error(SVTAD_ERR_UNSUPPORTED, "grad_clip: out of host memory");
     const ClipPlan plan{tensors, count};
     const int64_t parts = plan.parts();
     if (parts > INT32_MAX) return set_error(SVTAD_ERR_UNSUPPORTED, "grad_clip: too many tensors");
@@ -304,10 +376,9 @@ extern "C" int svtad_grad_clip(const svtad_grad* tensors, int64_t count, int nor
     }
     // the last launch's tensors first: the cache holds them still
     for (int i = n_starts - 1; i >= 0; --i) {
-        int64_t at = starts[i];
-        const int64_t stop = i + 1 < n_starts ? starts[i + 1] : count;
-        while (at < stop) {
-            at = plan.take(at, l);
+        const ClipPlan part{tensors, i + 1 < n_starts ? starts[i + 1] : count, memory == Shared::kRepeats};
+        for (int64_t at = starts[i]; at < part.count;) {
+            at = part.take(at, l);
             if (!l.count) continue;
             const int grid = clip_groups(l.end[l.count - 1], 2 * kMaxGroups);
             if (l.g_type == SVTAD_F32) launch_scale<float>(l, s, grid, hs);

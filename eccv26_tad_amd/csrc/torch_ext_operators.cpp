@@ -282,9 +282,19 @@ at::Tensor op_grad_clip(const std::vector<at::Tensor>& grads, const c10::optiona
         check_float(t, "gradients");
         TORCH_CHECK(t.device() == grads[0].device(), "opentad_sparse_ops.grad_clip: gradients must be on one device");
         if (!t.is_non_overlapping_and_dense()) {
-            t = t.contiguous();
-            copies.push_back(t);
-            if (!apart) copied.push_back(i);
+            // one copy for all mentions of a tensor, which is scaled once for each
+            const auto is_t = [&t](const at::Tensor& u) {
+                return u.data_ptr() == t.data_ptr() && u.scalar_type() == t.scalar_type() && u.sizes() == t.sizes() &&
+                       u.strides() == t.strides();
+            };
+            size_t same = 0;
+            while (same < copied.size() && !is_t(grads[copied[same]])) ++same;
+            if (same < copied.size()) t = copies[same];
+            else {
+                t = t.contiguous();
+                copies.push_back(t);
+                if (!apart) copied.push_back(i);
+            }
         }
         list[i].g = t.data_ptr(), list[i].count = t.numel(), list[i].g_type = dtype_code(t);
         if (!write) continue;

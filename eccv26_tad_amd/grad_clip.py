@@ -36,7 +36,9 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float 
 
     ``grads`` is a sequence of float16, bfloat16 or float32 tensors on one GPU;
     ``scale`` removes a loss scale in the same pass. Norms are summed in float64
-    over all tensors, in a fixed order. A norm of NaN makes every gradient NaN
+    over all tensors, in a fixed order. A gradient that is listed twice counts and
+    is scaled once per mention; a tensor of ``out`` shares no memory with another
+    tensor. A norm of NaN makes every gradient NaN
     and an infinite one zeros and NaN, as ``torch`` has it."""
     max_norm = float(max_norm)
     if not max_norm >= 0:

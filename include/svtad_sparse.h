@@ -731,8 +731,10 @@ int svtad_cross_attention_bwd(const svtad_cross_args* args, const void* out, con
  * Gradient clipping over `count` tensors (host array of descriptors; dense
  * elements, any mix of types). norm[0] = |scale| * (2-norm of all elements, or
  * their largest magnitude); with `write`, out = g * scale * min(1, max_norm /
- * (norm + 1e-6)), rounded once to out_type; out may be g. A negative max_norm
- * scales without a limit. Squares are summed in float64 in a fixed order.
+ * (norm + 1e-6)), rounded once to out_type; out may be g (of one type). Tensors in
+ * place may share memory with one another (one listed twice counts twice in the
+ * norm and is scaled twice); an output apart shares none with any other tensor. A
+ * negative max_norm scales without a limit. Squares are summed in float64 in a fixed order.
  */
 enum svtad_grad_norm { SVTAD_NORM_2 = 0, SVTAD_NORM_INF = 1 };
 typedef struct {

@@ -221,3 +221,58 @@ def test_refusals(dev):
         sv.clip_grads(g, 1.0, out=[torch.ones(5, device=dev)])
     with pytest.raises(RuntimeError, match="no tensors"):
         sv.grad_norm([])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_gradients_listed_more_than_once(dev, dtype):
+    """A shared parameter's gradient counts and is scaled once per mention, one
+    tensor after the other, and so are views that share some elements."""
+    import eccv26_tad_amd as sv
+
+    T = DTYPES[dtype]
+    big, small, strided = _grads(dev, T, [(700, 999), (5,), (60, 80)])
+    lists = [big, small, big, strided[:, ::2], small, strided[:, ::2], big]
+    before = [g.clone() for g in lists]
+    n = _norm(before)
+    keep = strided.clone()
+    got = sv.clip_grads(lists, n / 2)
+    assert abs(float(got) - n) <= NORM_TOL * n
+    c = n / 2 / (n + 1e-6)
+    # each of the m products is rounded: m roundings of a value that only shrinks
+    for g, m, was in ((big, 3, before[0]), (small, 2, before[1]), (strided[:, ::2], 2, before[3])):
+        want = was.double() * c ** m
+        assert bool(((g.double() - want).abs() <= m * (U[T] * want.abs() + torch.finfo(T).smallest_normal * 2.0 ** -9)).all())
+    assert torch.equal(strided[:, 1::2], keep[:, 1::2])
+    flat = _grads(dev, T, [(300000,)])[0]
+    a, b, was = flat[:200000], flat[100000:], flat.clone()
+    n = _norm([a, b])
+    sv.clip_grads([a, b], n / 4)
+    c = n / 4 / (n + 1e-6)
+    want = was.double() * c
+    want[100000:200000] *= c
+    assert bool(((flat.double() - want).abs() <= 2 * (U[T] * want.abs() + torch.finfo(T).smallest_normal * 2.0 ** -9)).all())
+
+
+def test_a_shared_parameter_as_torch(dev):
+    import eccv26_tad_amd as sv
+
+    p, q = (torch.nn.Parameter(torch.zeros(300, 500, device=dev)) for _ in range(2))
+    p.grad, = _grads(dev, torch.float32, [(300, 500)])
+    q.grad = p.grad.clone()
+    want = torch.nn.utils.clip_grad_norm_([p, p], 1.0, foreach=False)
+    got = sv.clip_grad_norm_([q, q], 1.0)
+    assert abs(float(got) - float(want)) <= 1e-5 * float(want)
+    assert float((q.grad - p.grad).norm()) <= 1e-5 * float(p.grad.norm())
+
+
+def test_outputs_that_share_memory_are_refused(dev):
+    import eccv26_tad_amd as sv
+
+    grads = _grads(dev, torch.float32, [(100,), (100,)])
+    buf = torch.full((300,), 7.0, device=dev)
+    for out in ([buf[:100], buf[50:150]], [buf[:100], buf[:100]], [buf[:100], grads[0]], [grads[0], grads[0]]):
+        with pytest.raises(RuntimeError, match="shares memory"):
+            sv.clip_grads(grads, 1.0, out=out)
+    assert bool((buf == 7.0).all())
+    sv.clip_grads([grads[0], grads[0]], 1.0, out=[buf[:100], buf[100:200]])  # read twice, written once each
+    assert torch.equal(buf[:100], buf[100:200]) and bool((buf[200:] == 7.0).all())

@@ -166,3 +166,22 @@ def test_cross_attention_bwd_without_queries(lib):
     for given in (dict(), dict(k=16), dict(v=16)):
         assert bwd(**given) == INVALID and b"NULL" in lib.svtad_last_error()
     assert bwd(batch=0) == OK
+
+
+def test_grad_clip_shared_memory(lib):
+    """An output that shares memory with another tensor is refused; gradients in
+    place may share it with one another."""
+
+    def call(*tensors, write=1):
+        arr, norm = (Grad * len(tensors))(*tensors), (ctypes.c_float * 1)()
+        return lib.svtad_grad_clip(arr, I64(len(tensors)), 0, F(1.0), F(1.0), write, norm, None, ctypes.c_size_t(0), None)
+
+    A, B, C = 4096, 8192, 16384  # 1000 float32 elements from each on do not meet
+    at = lambda g, out=None, n=1000, to=F32: Grad(g, g if out is None else out, n, F32, to)  # noqa: E731
+    for good in ((at(A), at(A)), (at(B), at(A, n=1025), at(C)), (at(A, C), at(A, B)), (at(B, C), at(A)),
+                 (at(A, C), at(B, C + 4000))):
+        assert call(*good) == WORKSPACE
+    for bad in ((at(A, C), at(B, C)), (at(A, B), at(B, C)), (at(B, C), at(A, B)), (at(A), at(A, C)), (at(A, C), at(C)),
+                (at(A, A + 4),), (at(A, B), at(C, B + 3996)), (at(A, A, to=F16),)):
+        assert call(*bad) == INVALID and b"shares memory" in lib.svtad_last_error()
+        assert call(*bad, write=0) == WORKSPACE

@@ -314,3 +314,52 @@ def test_refusals(dev):
         sv.cross_attention(q, k, v, key_mask=torch.ones(2, 5, dtype=torch.bool, device=dev))
     with no("key_mask"):
         sv.cross_attention(q, k, v, key_mask=torch.ones(2, 6, device=dev))
+
+
+def _check_gradients(dev, q, k, v, dout, rows=False):
+    """Gradients in float16 against float64. Beside the relative roundings of
+    `_check` stands the result's own below the type's normal range: half of
+    2^-24, its spacing there. With `rows` every query's dq is held to its own
+    size."""
+    import eccv26_tad_amd as sv
+
+    ls = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    got = torch.autograd.grad(sv.cross_attention(*ls), ls, dout)
+    want, moved = _exact(q, k, v, dout, None, None, q.shape[-1] ** -0.5)
+    u = U[q.dtype]
+    for name, g, w, m in zip(("dq", "dk", "dv"), got, want[1:], moved[1:]):
+        assert float(w.abs().max()) < 6e4 and g.isfinite().all(), name
+        dims = (2, 3) if rows and name == "dq" else (0, 1, 2, 3)
+        size = lambda t: torch.linalg.vector_norm(t, dim=dims)  # noqa: E731
+        count = w[0, 0].numel() if rows and name == "dq" else w.numel()
+        allow = 3 * u * (size(w) + (0 if m is None else size(m))) + 2.0 ** -25 * math.sqrt(count)
+        off = size(g.double() - w)
+        assert bool((off <= allow).all()), (name, float((off / allow).max()))
+
+
+@pytest.mark.parametrize("gain", [1.0, 1e-2, 1e-3])
+@pytest.mark.parametrize("Nq,Nk", [(70, 20000), (2000, 8192), (1, 31361), (3000, 100)])
+def test_small_float16_gradients(dev, Nq, Nk, gain):
+    """A score gradient among n keys is near 1 / n of dout, below float16's normal
+    values where dout is not."""
+    q, k, v, dout = _inputs(dev, 1, Nq, Nk, 2, 2, 32, torch.float32, seed=1)
+    _check_gradients(dev, q.half(), k.half(), v.half(), (gain * dout).half())
+
+
+@pytest.mark.parametrize("Nq,Nk", [(5, 3), (40, 150)])
+def test_large_float16_gradients(dev, Nq, Nk):
+    """Score gradients past float16's largest value, whose sums are within it."""
+    q, k, v, dout = _inputs(dev, 1, Nq, Nk, 2, 2, 128, torch.float32, seed=1)
+    # few keys, or scores so steep that few keys count: probabilities of order 1
+    q = q * (1 if Nk < 10 else 3)
+    _check_gradients(dev, q.half(), k.half(), (10 * v).half(), (1600 * dout / math.sqrt(Nq / 5)).half())
+
+
+def test_float16_gradients_of_many_sizes(dev):
+    """Queries whose gradients lie 4^9 apart, side by side in a tile, some zero;
+    and keys that are seen by large ones first or last."""
+    q, k, v, dout = _inputs(dev, 1, 300, 700, 2, 2, 32, torch.float32, seed=2)
+    size = 4.0 ** -(torch.arange(300, device=dev) % 10)
+    size[::17] = 0
+    for order in (size, size.sort().values, size.sort(descending=True).values):
+        _check_gradients(dev, q.half(), k.half(), v.half(), (100 * dout * order[None, :, None, None]).half(), rows=True)

@@ -38,6 +38,13 @@ constexpr float kNegInf = -__builtin_huge_valf();
 // float32 sums and the operand types hold as well as those below 1.
 constexpr float kSlack = 8.f;
 
+// What sums relative to the maximum m are multiplied by to be relative to `top`, at
+// least m. Parts with one maximum are added as they are, -inf included: no score of
+// theirs was above it, but one may be NaN, and so may their sums.
+__device__ __forceinline__ float power_of(float m, float top, float c) {
+    return m == top ? 1.f : __builtin_amdgcn_exp2f((m - top) * c);
+}
+
 // Keys of a staged tile: 64, or 32 per wave where the waves share a tile.
 template <int WM> constexpr int kTileKeys = WM == 1 ? 128 : 64;
 
@@ -256,26 +263,24 @@ __global__ __launch_bounds__(256, (kResidentFwd<T, DP>)) void k_cross_fwd(CrossA
         float top = m;
 #pragma unroll
         for (int w = 1; w < WK; ++w) top = fmaxf(top, jm[(w * ROWS + at) * 2]);
-        if (top != kNegInf) {
-            float f = __builtin_amdgcn_exp2f((m - top) * p.c);
-            l *= f;
+        float f = power_of(m, top, p.c);
+        l *= f;
 #pragma unroll
-            for (int db = 0; db < DB; ++db) acc[db] *= f;
+        for (int db = 0; db < DB; ++db) acc[db] *= f;
 #pragma unroll
-            for (int w = 1; w < WK; ++w) {
-                f = __builtin_amdgcn_exp2f((jm[(w * ROWS + at) * 2] - top) * p.c);
-                l += f * jm[(w * ROWS + at) * 2 + 1];
+        for (int w = 1; w < WK; ++w) {
+            f = power_of(jm[(w * ROWS + at) * 2], top, p.c);
+            l += f * jm[(w * ROWS + at) * 2 + 1];
 #pragma unroll
-                for (int db = 0; db < DB; ++db)
+            for (int db = 0; db < DB; ++db)
 #pragma unroll
-                    for (int q = 0; q < M::Q; ++q) {
-                        const f32x4 v = *(const f32x4*)(jo + (w * ROWS + at) * DA + db * S + M::row4(q, lane));
+                for (int q = 0; q < M::Q; ++q) {
+                    const f32x4 v = *(const f32x4*)(jo + (w * ROWS + at) * DA + db * S + M::row4(q, lane));
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[db][4 * q + e] += v[e] * f;
-                    }
-            }
-            m = top;
+                    for (int e = 0; e < 4; ++e) acc[db][4 * q + e] += v[e] * f;
+                }
         }
+        m = top;
     }
 
     if (r >= p.M) return;
@@ -339,15 +344,13 @@ __global__ __launch_bounds__(256) void k_cross_join(CrossArgs p) {
 #pragma unroll
         for (int q = 0; q < G; ++q) top = fmaxf(top, red[q][j.chunk][0]);
     }
-    if (top != kNegInf) {
 #pragma unroll
-        for (int i = 0; i < kMost; ++i)
-            if (s0 + i < s1) {
-                const float f = __builtin_amdgcn_exp2f((m[i] - top) * p.c);
-                l += f * w[i];
-                acc += v[i] * f;
-            }
-    }
+    for (int i = 0; i < kMost; ++i)
+        if (s0 + i < s1) {
+            const float f = power_of(m[i], top, p.c);
+            l += f * w[i];
+            acc += v[i] * f;
+        }
     if constexpr (G > 1) red[j.g][j.chunk][1] = l;
     acc = join_groups<G>(acc, j);  // its barrier covers red
     if (j.g != 0 || !in) return;

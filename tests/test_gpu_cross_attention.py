@@ -363,3 +363,33 @@ def test_float16_gradients_of_many_sizes(dev):
     size[::17] = 0
     for order in (size, size.sort().values, size.sort(descending=True).values):
         _check_gradients(dev, q.half(), k.half(), v.half(), (100 * dout * order[None, :, None, None]).half(), rows=True)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("Nq,Nk", [(1, 9), (3, 20000), (20, 200), (70, 300)])
+def test_nan_of_a_query_or_a_seen_key_is_kept(dev, Nq, Nk, masked, dtype):
+    """It reaches the results of its query, or of its sample and key head, and no others."""
+    import eccv26_tad_amd as sv
+
+    q, k, v, _ = _inputs(dev, 2, Nq, Nk, 4, 2, 32, DTYPES[dtype])
+    mask = None
+    if masked:
+        mask = torch.zeros(2, Nk, dtype=torch.bool, device=dev)
+        mask[:, Nk - 2 :] = True
+    want = sv.cross_attention(q, k, v, key_mask=mask)
+    bad = q.clone()
+    bad[0, Nq - 1, 1] = math.nan
+    got = sv.cross_attention(bad, k, v, key_mask=mask)
+    hit = torch.zeros_like(q, dtype=torch.bool)
+    hit[0, Nq - 1, 1] = True
+    assert bool(got[hit].isnan().all()) and torch.equal(got[~hit], want[~hit])
+    bad = k.clone()
+    bad[1, Nk - 2, 0, 3] = math.nan
+    if masked:
+        mask[:, Nk - 1] = False  # one key alone is seen
+        want = sv.cross_attention(q, k, v, key_mask=mask)
+    got = sv.cross_attention(q, bad, v, key_mask=mask)
+    hit = torch.zeros_like(q, dtype=torch.bool)
+    hit[1, :, :2] = True
+    assert bool(got[hit].isnan().all()) and torch.equal(got[~hit], want[~hit])

@@ -103,7 +103,9 @@ __global__ __launch_bounds__(256, (kResidentBwd<T, DP>)) void k_cross_bwd_q(Cros
     }
     constexpr bool kScaled = std::is_same_v<T, f16>;
     GradScale gs;
+    // +inf: the row sees no key, and has no gradient whatever dout and q hold
     float lse = in ? p.lse[bh * p.M + r] : -kNegInf;  // past the end: probabilities 0
+    const bool none = lse == -kNegInf;
     if constexpr (kScaled) lse -= gs.e;  // probabilities, and with them the score gradients, times 2^e
     if (in && slot == 0 && wk == 0 && split == 0) p.delta[bh * p.M + r] = -delta;
     if (!p.out) return;
@@ -158,6 +160,10 @@ __global__ __launch_bounds__(256, (kResidentBwd<T, DP>)) void k_cross_bwd_q(Cros
         const float f = gs.undo();
 #pragma unroll
         for (int db = 0; db < DB; ++db) acc[db] *= f;
+    }
+    if (none) {
+#pragma unroll
+        for (int db = 0; db < DB; ++db) acc[db] = M::fill(0.f);
     }
 
     if constexpr (WK > 1) {  // add the waves of equal rows, in order

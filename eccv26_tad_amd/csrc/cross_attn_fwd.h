@@ -20,7 +20,9 @@
 // 620 us, 0.81 to 0.65 PFLOP/s with the clock), by memory where there are few (one
 // query over 8 x 31361 keys of 4 heads: 36 us, 4.8 TB/s).
 // Keys that are not seen are staged as zeros and their scores replaced, so
-// neither infinities nor NaN in their places reach a result.
+// neither infinities nor NaN in their places reach a result. A sample's rows whose
+// keys are all unseen are set to zero at the end: a product of zeros with a row's
+// own infinities or NaN is no zero.
 #pragma once
 
 #include "cross_attn.h"
@@ -113,6 +115,16 @@ struct KeyTiles {
         sk.store(keys(tile));
         sv.store(values(tile));
         landed();
+    }
+
+    // Whether the mask shows any key of this split (the same for the wave). It is read
+    // again where that matters: a flag kept through the walk cost the kernel of many
+    // rows 6 spilled registers.
+    __device__ __forceinline__ bool any(const CrossArgs& p) const {
+        const int64_t end = lesser<int64_t>(len, t1 * TK);
+        bool in = false;
+        for (int64_t n = t0 * TK + (threadIdx.x & 63); n < end; n += 64) in |= mask[n * p.mask_n] != 0;
+        return __any(in);
     }
 
     // All tiles of this split: whole(tile) on those whose keys are all seen,
@@ -242,6 +254,11 @@ __global__ __launch_bounds__(256, (kResidentFwd<T, DP>)) void k_cross_fwd(CrossA
     };
     keys.walk(p, [&](int64_t t) { use(t, std::false_type()); }, [&](int64_t t) { use(t, std::true_type()); });
     l = M::col_sum(l);
+    if (keys.mask && __any(l != l) && !keys.any(p)) {
+        m = kNegInf, l = 0.f;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) acc[db] = M::fill(0.f);
+    }
 
     if constexpr (WK > 1) {  // join the waves of equal rows, in order
         constexpr int DA = DB * S;

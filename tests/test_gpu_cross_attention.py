@@ -393,3 +393,34 @@ def test_nan_of_a_query_or_a_seen_key_is_kept(dev, Nq, Nk, masked, dtype):
     hit = torch.zeros_like(q, dtype=torch.bool)
     hit[1, :, :2] = True
     assert bool(got[hit].isnan().all()) and torch.equal(got[~hit], want[~hit])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("Nq,Nk", [(1, 700), (20, 200), (150, 130), (3, 20000), (2000, 90)])
+@pytest.mark.parametrize("kind", ["lengths", "mask", "both"])
+def test_queries_without_keys_may_hold_anything(dev, Nq, Nk, kind, dtype):
+    """Queries and upstream gradients of a sample whose keys are all hidden, by a
+    length or by the mask: zeros, whatever they hold, and the other samples' bits
+    stay."""
+    T = DTYPES[dtype]
+    q, k, v, dout = _inputs(dev, 3, Nq, Nk, 4, 2, 32, T)
+    lengths = torch.tensor([Nk, 0, Nk - 1], dtype=torch.int32, device=dev) if kind == "lengths" else None
+    mask = None
+    if kind != "lengths":
+        mask = torch.rand(3, Nk, device=dev, generator=torch.Generator(device=dev).manual_seed(6)) < 0.5
+        mask[:, 0] = True
+        mask[1] = False
+        if kind == "both":  # only the keys past the length are seen
+            lengths = torch.tensor([Nk, Nk // 2, Nk - 1], dtype=torch.int32, device=dev)
+            mask[1, Nk // 2 :] = True
+    want = _check(q, k, v, dout, lengths, mask)
+    for bad_q, bad_g in ((math.nan, 1.0), (math.inf, 1.0), (1.0, math.nan), (1.0, -math.inf), (-math.inf, math.inf)):
+        import eccv26_tad_amd as sv
+
+        q2, g2 = q.clone(), dout.clone()
+        q2[1], g2[1] = q2[1] * bad_q, g2[1] * bad_g
+        ls = [t.detach().requires_grad_(True) for t in (q2, k, v)]
+        out = sv.cross_attention(*ls, key_lengths=lengths, key_mask=mask)
+        got = (out.detach(), *torch.autograd.grad(out, ls, g2))
+        for name, a, b in zip(("out", "dq", "dk", "dv"), got, want):
+            assert not a[1].any() and torch.equal(a, b), (name, bad_q, bad_g)

@@ -32,7 +32,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_lengt
 
     Softmax statistics and sums are float32; probabilities are rounded to the
     inputs' dtype as operands of the matrix units. Gradients come without
-    atomics: equal inputs give equal bits."""
+    atomics: equal inputs give equal bits. Differentiable once, in reverse mode;
+    a second derivative and forward mode raise."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
     if key_lengths is not None and key_lengths.dtype == torch.int64:

@@ -10,8 +10,12 @@
 
 namespace {
 
+// Also that no tangent of forward-mode differentiation comes with it, which these
+// functions would drop in silence.
 void check_float(const at::Tensor& t, const char* name) {
     check_gpu(t, name);
+    TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), "opentad_sparse_ops: forward-mode differentiation is not supported (",
+                                name, " has a tangent)");
     const auto st = t.scalar_type();
     TORCH_CHECK(st == at::kFloat || st == at::kHalf || st == at::kBFloat16, "opentad_sparse_ops: ", name,
                 " must be float32, float16 or bfloat16, got ", st);
@@ -240,6 +244,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> op_cross_attention_bwd(
     const at::Tensor& lse, const c10::optional<at::Tensor>& rest, const c10::optional<at::Tensor>& lengths,
     const c10::optional<at::Tensor>& mask, double scale, bool need_q, bool need_kv) {
     CrossCall c = cross_call(q, k, v, lengths, mask, scale, "cross_attention_bwd");
+    check_float(dout_in, "dout");
     const bool has_rest = rest.has_value() && rest->defined();
     for (const at::Tensor* t : {&dout_in, &out, has_rest ? &*rest : &out})
         TORCH_CHECK(t->sizes() == q.sizes() && t->scalar_type() == q.scalar_type() && t->device() == q.device(),
@@ -418,14 +423,21 @@ struct CrossAttentionNode : torch::autograd::Function<CrossAttentionNode> {
 
 }  // namespace
 
-// layer_norm and cross_attention as differentiable functions
+// layer_norm and cross_attention as differentiable functions. A tangent is refused
+// here: within the node's forward, forward mode is off and none is seen.
 at::Tensor op_layer_norm_grad(const at::Tensor& x, const c10::optional<at::Tensor>& w, const c10::optional<at::Tensor>& b,
                               double eps) {
+    check_float(x, "x");
+    for (const auto* p : {&w, &b})
+        if (p->has_value() && (*p)->defined()) check_float(**p, "weight and bias");
     return LayerNormNode::apply(x, w, b, eps);
 }
 at::Tensor op_cross_attention_grad(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                                    const c10::optional<at::Tensor>& lengths, const c10::optional<at::Tensor>& mask,
                                    double scale) {
+    check_float(q, "q");
+    check_float(k, "k");
+    check_float(v, "v");
     return CrossAttentionNode::apply(q, k, v, lengths, mask, scale);
 }
 

@@ -20,7 +20,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     has its dtype, also under autocast (where ``torch`` returns float32).
     ``weight`` and ``bias`` are ``[channels]``, in x's dtype or float32 (any
     other is widened to float32), or None. Their gradients are summed over all
-    rows in float32 in a fixed order and rounded once."""
+    rows in float32 in a fixed order and rounded once. Differentiable once, in
+    reverse mode; a second derivative and forward mode raise."""
     given = [p for p in (weight, bias) if p is not None]
     if any(p.dtype not in (x.dtype, torch.float32) for p in given) or len({p.dtype for p in given}) > 1:
         weight, bias = (None if p is None else p.float() for p in (weight, bias))

@@ -204,3 +204,36 @@ def test_second_derivative_is_never_partial(dev):
     (g,) = torch.autograd.grad((sv.cross_attention(q, k, k) * q).sum(), q, create_graph=True)
     with pytest.raises(RuntimeError, match="cross_attention twice"):
         torch.autograd.grad(g.sum(), k)
+
+
+def test_forward_mode_raises(dev):
+    """A tangent is not carried by these operators: it raises, with gradients on or
+    off, in the operator, in its backward and in the clipping of gradients."""
+    import torch.autograd.forward_ad as fw
+
+    import eccv26_tad_amd as sv
+
+    x, w = torch.randn(5, 64, device=dev), torch.rand(64, device=dev)
+    q, k = torch.randn(1, 5, 2, 16, device=dev), torch.randn(1, 7, 2, 16, device=dev)
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))  # noqa: E731
+        calls = [lambda: sv.layer_norm(dual(x), w), lambda: sv.layer_norm(x, dual(w)), lambda: sv.layer_norm(x, w, dual(w)),
+                 lambda: sv.layer_norm(dual(x.clone().requires_grad_(True)), w),
+                 lambda: sv.cross_attention(dual(q), k, k), lambda: sv.cross_attention(q, dual(k), k),
+                 lambda: sv.cross_attention(q, k, dual(k)), lambda: sv.cross_attention(dual(q), k.clone().requires_grad_(True), k),
+                 lambda: sv.clip_grads([x.clone(), dual(x)], 1.0), lambda: sv.grad_norm([dual(x)])]
+        for i, call in enumerate(calls):
+            for context in (torch.enable_grad, torch.no_grad):
+                with context(), pytest.raises((RuntimeError, NotImplementedError)):
+                    call()
+                    pytest.fail(f"call {i} dropped a tangent")
+        y = sv.layer_norm(x.clone().requires_grad_(True), w)
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            y.backward(dual(torch.ones_like(y)))
+            pytest.fail("the norm's backward dropped a tangent")
+        out = sv.cross_attention(q.clone().requires_grad_(True), k, k)
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            out.backward(dual(torch.ones_like(out)))
+            pytest.fail("the attention's backward dropped a tangent")
+        # without a tangent all is as outside
+        assert torch.equal(sv.layer_norm(x, w), sv.layer_norm(x.clone().requires_grad_(True), w))

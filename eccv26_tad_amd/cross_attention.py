@@ -13,6 +13,7 @@ import torch
 import torch.nn as nn
 
 from . import opentad_sparse_ops as _ops
+from .adapter import _is_plain
 from .layer_norm import layer_norm
 
 
@@ -73,7 +74,11 @@ class CrossAttention(nn.Module):
 
     @staticmethod
     def _norm(layer, x):
-        return layer_norm(x, layer.weight, layer.bias, layer.eps)
+        """The layer's norm in x's dtype. A layer whose call does more than compute
+        it, or another layer in its place, is called."""
+        if _is_plain(layer, nn.LayerNorm) and layer.normalized_shape == x.shape[-1:]:
+            return layer_norm(x, layer.weight, layer.bias, layer.eps)
+        return layer(x).to(x.dtype)
 
     def project_context(self, context: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """Keys (normalised) and values ``[B, Nk, kv_heads, head_dim]`` of a context."""

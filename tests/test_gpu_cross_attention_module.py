@@ -237,3 +237,63 @@ def test_forward_mode_raises(dev):
             pytest.fail("the attention's backward dropped a tangent")
         # without a tangent all is as outside
         assert torch.equal(sv.layer_norm(x, w), sv.layer_norm(x.clone().requires_grad_(True), w))
+
+
+NORMS = ["norm", "context_norm", "q_norm", "k_norm"]
+
+
+@pytest.mark.parametrize("autocast", [False, True])
+@pytest.mark.parametrize("which", NORMS)
+def test_norms_are_called_where_a_call_does_more(dev, which, autocast):
+    """Hooks on a norm run, a replaced forward or another layer in its place is
+    taken; otherwise the kernels compute the same."""
+    import eccv26_tad_amd as sv
+
+    torch.manual_seed(4)
+    m = sv.CrossAttention(64, 2, context_dims=48, kv_heads=1).to(dev)
+    x, c = torch.randn(2, 5, 64, device=dev), torch.randn(2, 30, 48, device=dev)
+
+    def run():
+        with torch.autocast("cuda", dtype=torch.bfloat16, enabled=autocast):
+            return m(x, c)
+
+    tol = 12 * 2.0 ** -8 if autocast else 1e-5
+    want, layer, calls = run(), getattr(m, which), []
+    handle = layer.register_forward_hook(lambda mod, a, out: calls.append(which))
+    assert _rel(run(), want.double()) <= tol and calls == [which]
+    handle.remove()
+    handle = layer.register_forward_pre_hook(lambda mod, a: (2 * a[0],))
+    twice = run()
+    handle.remove()
+    layer.forward = lambda t: torch.nn.LayerNorm.forward(layer, 2 * t)
+    assert torch.equal(run(), twice)
+    del layer.forward
+    handle = torch.nn.modules.module.register_module_forward_hook(lambda mod, a, out: calls.append(mod))
+    run()
+    handle.remove()
+    assert layer in calls
+    assert torch.equal(run(), want)
+    setattr(m, which, torch.nn.Identity())
+    assert run().shape == want.shape
+    # without a norm before them the other layers see what it was given
+    seen = []
+    setattr(m, which, torch.nn.LayerNorm(layer.normalized_shape, elementwise_affine=False, device=dev))
+    getattr(m, which).register_forward_hook(lambda mod, a, out: seen.append(a[0]) or a[0])
+    hooked = run()
+    setattr(m, which, torch.nn.Identity())
+    assert len(seen) == 1 and torch.equal(run(), hooked)
+
+
+def test_hooked_norm_gradients(dev):
+    import eccv26_tad_amd as sv
+
+    torch.manual_seed(5)
+    m = sv.CrossAttention(64, 2).to(dev)
+    x = torch.randn(1, 5, 64, device=dev)
+    g = torch.randn(1, 5, 64, device=dev)
+    want = torch.autograd.grad(m(x, x), list(m.parameters()), g)
+    for n in NORMS:
+        getattr(m, n).register_forward_hook(lambda mod, a, out: None)
+    got = torch.autograd.grad(m(x, x), list(m.parameters()), g)
+    for (n, _), a, b in zip(m.named_parameters(), got, want):
+        assert n == "k_norm.bias" or _rel(a, b.double()) <= 1e-4, n

@@ -424,3 +424,28 @@ def test_queries_without_keys_may_hold_anything(dev, Nq, Nk, kind, dtype):
         got = (out.detach(), *torch.autograd.grad(out, ls, g2))
         for name, a, b in zip(("out", "dq", "dk", "dv"), got, want):
             assert not a[1].any() and torch.equal(a, b), (name, bad_q, bad_g)
+
+
+def test_stride_of_an_axis_of_one(dev):
+    """What stride an axis with one place has is no matter."""
+    import eccv26_tad_amd as sv
+
+    q, k, v, _ = _inputs(dev, 1, 1, 1, 1, 1, 32, torch.float16)
+    far = lambda t: t.as_strided(t.shape, (1 << 40, 1 << 40, 1 << 40, 1))  # noqa: E731
+    assert torch.equal(sv.cross_attention(far(q), far(k), far(v)), sv.cross_attention(q, k, v))
+    q, k, v, dout = _inputs(dev, 1, 1, 90, 4, 2, 32, torch.bfloat16)
+    one = q.as_strided(q.shape, (0, 1 << 30, 32, 1))
+    want = _check(q, k, v, dout)
+    assert all(torch.equal(a, b) for a, b in zip(_check(one, k, v, dout.as_strided(q.shape, (0, 1 << 30, 32, 1))), want))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_masks_of_any_strides(dev, dtype):
+    """One mask for all samples, every other place of a wider one, and the
+    transpose of [keys, samples]."""
+    q, k, v, dout = _inputs(dev, 3, 20, 150, 2, 2, 32, DTYPES[dtype])
+    wide = torch.rand(3, 300, device=dev, generator=torch.Generator(device=dev).manual_seed(3)) < 0.6
+    turned = wide[:, :150].t().contiguous().t()
+    for mask in (wide[:1, :150].expand(3, 150), wide[:, ::2], turned, wide[:, :1].expand(3, 150)):
+        got, want = (_check(q, k, v, dout, None, m) for m in (mask, mask.contiguous()))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -185,3 +185,14 @@ def test_grad_clip_shared_memory(lib):
                 (at(A, A + 4),), (at(A, B), at(C, B + 3996)), (at(A, A, to=F16),)):
         assert call(*bad) == INVALID and b"shares memory" in lib.svtad_last_error()
         assert call(*bad, write=0) == WORKSPACE
+
+
+def test_cross_attention_stride_of_an_axis_of_one(lib):
+    Z = ctypes.c_size_t(0)
+    call = lambda **kw: lib.svtad_cross_attention(_cross(**kw), None, None, None, None, Z, F16, None)  # noqa: E731
+    far = 1 << 40
+    for given in (dict(nq=1, q_stride=[128, far, 32]), dict(nq=1, q_stride=[128, -far, 32]),
+                  dict(nk=1, k_stride=[64, far, 32], v_stride=[64, far, 32]),
+                  dict(heads=1, kv_heads=1, q_stride=[320, 32, far], k_stride=[640, 32, far], v_stride=[640, 32, -far])):
+        assert call(**given) == INVALID and b"NULL" in lib.svtad_last_error()
+    assert call(nq=2, q_stride=[128, far, 32]) == UNSUPPORTED

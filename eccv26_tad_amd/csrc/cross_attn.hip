@@ -75,11 +75,22 @@ static size_t bwd_bytes(const svtad_cross_args& a, int dtype) {
     return align256((size_t)all_rows(a) * 4) + std::max(pq, pk);
 }
 
+// The strides of a tensor [batch, tokens, heads, .] as the kernels take them: that of
+// an axis with one place, which may be any number, as 0.
+struct Strides {
+    int64_t b, n, h;
+};
+static Strides strides(const int64_t* s, int64_t batch, int64_t tokens, int heads) {
+    return {batch > 1 ? s[0] : 0, tokens > 1 ? s[1] : 0, heads > 1 ? s[2] : 0};
+}
+static Strides q_strides(const svtad_cross_args& a, const int64_t* s) { return strides(s, a.batch, a.nq, a.heads); }
+static Strides k_strides(const svtad_cross_args& a, const int64_t* s) { return strides(s, a.batch, a.nk, a.kv_heads); }
+
 // Offsets within a tile of 128 tokens, over the heads of one key head, are 32
 // bits in the kernels.
-static bool near_strides(const int64_t* s, int group, int dtype) {
+static bool near_strides(const Strides& s, int group, int dtype) {
     const double size = dtype == SVTAD_F32 ? 4 : 2;
-    return s[1] >= 0 && s[2] >= 0 && ((double)s[1] * 128 + (double)s[2] * group + 128) * size < 2147483648.0;
+    return s.n >= 0 && s.h >= 0 && ((double)s.n * 128 + (double)s.h * group + 128) * size < 2147483648.0;
 }
 
 static int cross_check(const svtad_cross_args* a, int dtype) {
@@ -98,24 +109,25 @@ static int cross_check(const svtad_cross_args* a, int dtype) {
         bk * std::max(m, (double)a->nk) * 64 > (double)INT32_MAX * 64)
         return set_error(SVTAD_ERR_UNSUPPORTED, "cross_attention: too many rows or keys for one launch");
     const int g = a->heads / a->kv_heads;
-    if (!near_strides(a->q_stride, g, dtype) || !near_strides(a->k_stride, 1, dtype) || !near_strides(a->v_stride, 1, dtype))
+    if (!near_strides(q_strides(*a, a->q_stride), g, dtype) || !near_strides(k_strides(*a, a->k_stride), 1, dtype) ||
+        !near_strides(k_strides(*a, a->v_stride), 1, dtype))
         return set_error(SVTAD_ERR_UNSUPPORTED, "cross_attention: 128 tokens must lie within 2 GiB");
     return SVTAD_OK;
 }
 
 // Whether rows are read 16 bytes at a time: every start at 16 bytes and every
-// stride (of an axis with more than one place) a multiple of 8 elements.
-static bool whole_vectors(const svtad_cross_args& a, const void* p, const int64_t* s, int64_t tokens, int heads) {
-    return (uintptr_t)p % 16 == 0 && (a.batch <= 1 || s[0] % 8 == 0) && (tokens <= 1 || s[1] % 8 == 0) &&
-           (heads <= 1 || s[2] % 8 == 0);
+// stride a multiple of 8 elements.
+static bool whole_vectors(const void* p, const Strides& s) {
+    return (uintptr_t)p % 16 == 0 && s.b % 8 == 0 && s.n % 8 == 0 && s.h % 8 == 0;
 }
 
 static CrossArgs cross_args(const svtad_cross_args& a, int dtype) {
     CrossArgs p{};
     p.q = a.q, p.k = a.k, p.v = a.v;
-    p.qb = a.q_stride[0], p.qn = a.q_stride[1], p.qh = a.q_stride[2];
-    p.kb = a.k_stride[0], p.kn = a.k_stride[1], p.kh = a.k_stride[2];
-    p.vb = a.v_stride[0], p.vn = a.v_stride[1], p.vh = a.v_stride[2];
+    const Strides q = q_strides(a, a.q_stride), k = k_strides(a, a.k_stride), v = k_strides(a, a.v_stride);
+    p.qb = q.b, p.qn = q.n, p.qh = q.h;
+    p.kb = k.b, p.kn = k.n, p.kh = k.h;
+    p.vb = v.b, p.vn = v.n, p.vh = v.h;
     p.lengths = a.lengths;
     p.mask = a.mask, p.mask_b = a.mask_stride[0], p.mask_n = a.mask_stride[1];
     p.B = (int)a.batch, p.H = a.heads, p.KH = a.kv_heads, p.G = a.heads / a.kv_heads, p.D = a.head_dim;
@@ -123,8 +135,7 @@ static CrossArgs cross_args(const svtad_cross_args& a, int dtype) {
     p.scale = a.scale;
     p.c = (float)((double)a.scale * 1.4426950408889634);
     p.inv_g = 1.f / p.G;
-    p.vec = a.head_dim % 8 == 0 && whole_vectors(a, a.q, a.q_stride, a.nq, a.heads) &&
-            whole_vectors(a, a.k, a.k_stride, a.nk, a.kv_heads) && whole_vectors(a, a.v, a.v_stride, a.nk, a.kv_heads);
+    p.vec = a.head_dim % 8 == 0 && whole_vectors(a.q, q) && whole_vectors(a.k, k) && whole_vectors(a.v, v);
     p.up = p.down = 1.f;
     if (dtype == SVTAD_F16)
         for (int64_t n = 2; n <= a.nk && n <= 8192; n *= 2) p.up *= 2.f, p.down *= 0.5f;
@@ -195,10 +206,11 @@ extern "C" int svtad_cross_attention_bwd(const svtad_cross_args* a, const void* 
     p.rest = dtype == SVTAD_F32 ? nullptr : const_cast<void*>(rest);
     p.o = out, p.on = (int64_t)a->heads * a->head_dim, p.oh = a->head_dim, p.ob = a->nq * p.on;
     p.dout = dout;
-    if (dout_stride && !near_strides(dout_stride, p.G, dtype))
+    const Strides g = dout_stride ? q_strides(*a, dout_stride) : Strides{0, 0, 0};
+    if (!near_strides(g, p.G, dtype))
         return set_error(SVTAD_ERR_UNSUPPORTED, "cross_attention_bwd: 128 tokens of dout must lie within 2 GiB");
-    p.vec = p.vec && (uintptr_t)out % 16 == 0 && (uintptr_t)p.rest % 16 == 0 && (!dout_stride || whole_vectors(*a, dout, dout_stride, a->nq, a->heads));
-    if (dout_stride) p.gb = dout_stride[0], p.gn = dout_stride[1], p.gh = dout_stride[2];
+    p.vec = p.vec && (uintptr_t)out % 16 == 0 && (uintptr_t)p.rest % 16 == 0 && whole_vectors(dout, g);
+    p.gb = g.b, p.gn = g.n, p.gh = g.h;
     p.out = dq, p.dk = dk, p.dv = dv;
     p.lse = const_cast<float*>(lse);
     p.delta = (float*)workspace;

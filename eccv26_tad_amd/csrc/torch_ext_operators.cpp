@@ -164,9 +164,11 @@ struct CrossCall {
 };
 
 // t [batch, tokens, heads, head_dim] as the kernels read it: a strided last axis,
-// or 128 tokens that lie further apart than 2 GiB, are copied
+// or 128 tokens that lie further apart than 2 GiB, are copied (an axis with one place
+// may have any stride)
 at::Tensor readable(const at::Tensor& t, int64_t group) {
-    const double apart = ((double)t.stride(1) * 128 + (double)t.stride(2) * group + 128) * t.element_size();
+    const double n = t.size(1) > 1 ? t.stride(1) : 0, h = t.size(2) > 1 ? t.stride(2) : 0;
+    const double apart = (n * 128 + h * group + 128) * t.element_size();
     return (t.size(-1) <= 1 || t.stride(-1) == 1) && apart < 2147483648.0 ? t : t.contiguous();
 }
 

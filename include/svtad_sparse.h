@@ -696,8 +696,8 @@ int svtad_norm_bwd(const svtad_norm_args* args, const void* dy, void* dx, void* 
 
 /*
  * Cross attention: q [batch, nq, heads, head_dim] attends to k, v [batch, nk,
- * kv_heads, head_dim] (element strides of the first three axes given, the last
- * 1), head h to key head h / (heads / kv_heads). Sample b sees its first
+ * kv_heads, head_dim] (element strides of the first three axes given, any for an
+ * axis of one place, the last 1), head h to key head h / (heads / kv_heads). Sample b sees its first
  * lengths[b] keys (NULL: nk; clamped to 0 .. nk) where mask[b, n] is nonzero
  * (NULL: all). out [batch, nq, heads, head_dim] is dense. A row that sees no
  * key is 0 and has no gradient; what lies in unseen keys is never used.

@@ -8,6 +8,10 @@ namespace svtad {
 
 constexpr int kMaxHeadDim = 128;
 
+// Workgroups of one launch: with 256 threads each, the runtime takes a grid of 2^32
+// threads and more modulo 2^32, without an error.
+constexpr int64_t kMaxGrid = (1 << 24) - 1;
+
 // Splits of an axis of `tiles` tiles for `groups` workgroups of `rows` results:
 // as many as fill one, two, three or four workgroups per compute unit, or none,
 // whichever is estimated to take least. The estimate is in times of one tile on a
@@ -45,10 +49,12 @@ struct RowPlan {
     int wave_rows, splits;
 };
 
+static int row_tile(int64_t m) { return m <= 16 ? 16 : m <= 64 ? 64 : 128; }
+
 static RowPlan row_plan(const svtad_cross_args& a, int dtype) {
     const int64_t m = a.nq * (a.heads / a.kv_heads);
-    RowPlan r{m <= 16 ? 1 : m <= 64 ? 2 : 4, 1};
-    const int rows = r.wave_rows == 4 ? 128 : r.wave_rows == 2 ? 64 : 16;
+    const int rows = row_tile(m);
+    RowPlan r{rows == 128 ? 4 : rows == 64 ? 2 : 1, 1};
     r.splits = splits(a, dtype, cdiv(m, rows) * a.batch * a.kv_heads, cdiv(a.nk, r.wave_rows == 1 ? 128 : 64), rows, 2);
     return r;
 }
@@ -93,7 +99,7 @@ static bool near_strides(const Strides& s, int group, int dtype) {
     return s.n >= 0 && s.h >= 0 && ((double)s.n * 128 + (double)s.h * group + 128) * size < 2147483648.0;
 }
 
-static int cross_check(const svtad_cross_args* a, int dtype) {
+static int cross_check(const svtad_cross_args* a, int dtype, bool bwd) {
     if (!a) return set_error(SVTAD_ERR_INVALID, "cross_attention: args is NULL");
     if (dtype != SVTAD_F32 && dtype != SVTAD_F16 && dtype != SVTAD_BF16)
         return set_error(SVTAD_ERR_INVALID, "cross_attention: dtype must be float32, float16 or bfloat16");
@@ -106,7 +112,8 @@ static int cross_check(const svtad_cross_args* a, int dtype) {
         return set_error(SVTAD_ERR_INVALID, "cross_attention: scale must be positive and finite");
     const double m = (double)a->nq * (a->heads / a->kv_heads), bk = (double)a->batch * a->kv_heads;
     if ((m / 16 + 1) * bk * kMaxSplits > INT32_MAX || ((double)a->nk / 64 + 1) * bk * kMaxSplits > INT32_MAX ||
-        bk * std::max(m, (double)a->nk) * 64 > (double)INT32_MAX * 64)
+        bk * std::max(m, (double)a->nk) > (double)INT32_MAX || std::ceil(m / row_tile((int64_t)m)) * bk > kMaxGrid ||
+        (bwd && std::ceil((double)a->nk / kCrossKvKeys) * bk > kMaxGrid))
         return set_error(SVTAD_ERR_UNSUPPORTED, "cross_attention: too many rows or keys for one launch");
     const int g = a->heads / a->kv_heads;
     if (!near_strides(q_strides(*a, a->q_stride), g, dtype) || !near_strides(k_strides(*a, a->k_stride), 1, dtype) ||
@@ -148,16 +155,16 @@ static CrossArgs cross_args(const svtad_cross_args& a, int dtype) {
 using namespace svtad;
 
 extern "C" size_t svtad_cross_attention_workspace_bytes(const svtad_cross_args* a, int dtype) {
-    return cross_check(a, dtype) ? 0 : fwd_bytes(*a, dtype);
+    return cross_check(a, dtype, false) ? 0 : fwd_bytes(*a, dtype);
 }
 
 extern "C" size_t svtad_cross_attention_bwd_workspace_bytes(const svtad_cross_args* a, int dtype) {
-    return cross_check(a, dtype) ? 0 : bwd_bytes(*a, dtype);
+    return cross_check(a, dtype, true) ? 0 : bwd_bytes(*a, dtype);
 }
 
 extern "C" int svtad_cross_attention(const svtad_cross_args* a, void* out, float* lse, void* rest, void* workspace,
                                      size_t workspace_bytes, int dtype, void* stream) {
-    const int st = cross_check(a, dtype);
+    const int st = cross_check(a, dtype, false);
     if (st) return st;
     if (all_rows(*a) == 0) return SVTAD_OK;
     if (!a->q || !out || (a->nk > 0 && (!a->k || !a->v))) return set_error(SVTAD_ERR_INVALID, "cross_attention: NULL pointer");
@@ -191,7 +198,7 @@ static void cross_bwd(CrossArgs p, const svtad_cross_args& a, int dtype, hipStre
 extern "C" int svtad_cross_attention_bwd(const svtad_cross_args* a, const void* out, const void* rest, const float* lse,
                                          const void* dout, const int64_t* dout_stride, void* dq, void* dk, void* dv, void* workspace,
                                          size_t workspace_bytes, int dtype, void* stream) {
-    const int st = cross_check(a, dtype);
+    const int st = cross_check(a, dtype, true);
     if (st) return st;
     if (!dk != !dv) return set_error(SVTAD_ERR_INVALID, "cross_attention_bwd: dk and dv come together");
     if ((!dq && !dk) || a->batch == 0) return SVTAD_OK;

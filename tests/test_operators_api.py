@@ -196,3 +196,22 @@ def test_cross_attention_stride_of_an_axis_of_one(lib):
                   dict(heads=1, kv_heads=1, q_stride=[320, 32, far], k_stride=[640, 32, far], v_stride=[640, 32, -far])):
         assert call(**given) == INVALID and b"NULL" in lib.svtad_last_error()
     assert call(nq=2, q_stride=[128, far, 32]) == UNSUPPORTED
+
+
+def test_cross_attention_grids_within_the_runtimes(lib):
+    """2^24 workgroups of 256 threads are 2^32 threads, of which the runtime would
+    start none: a call that needs so many is refused."""
+    Z = ctypes.c_size_t(0)
+    call = lambda **kw: lib.svtad_cross_attention(_cross(**kw), None, None, None, None, Z, F16, None)  # noqa: E731
+    bwd = lambda **kw: lib.svtad_cross_attention_bwd(  # noqa: E731
+        _cross(**kw), None, None, None, None, None, None, P(16), P(16), None, Z, F16, None)
+    one = dict(heads=1, kv_heads=1, head_dim=8, q_stride=[8, 8, 8], k_stride=[8, 8, 8], v_stride=[8, 8, 8])
+    for sizes in (dict(batch=1 << 24, nq=1, nk=1), dict(batch=1 << 24, nq=16, nk=1), dict(batch=1 << 23, nq=129, nk=1),
+                  dict(batch=1 << 22, nq=400, nk=10)):
+        assert call(**one, **sizes) == UNSUPPORTED and b"too many" in lib.svtad_last_error()
+        assert bwd(**one, **sizes) == UNSUPPORTED
+    for sizes in (dict(batch=(1 << 24) - 1, nq=16, nk=1), dict(batch=(1 << 23) - 1, nq=17, nk=1)):
+        assert call(**one, **sizes) == INVALID and b"NULL" in lib.svtad_last_error()
+        assert bwd(**one, **sizes) == INVALID
+    keys = dict(batch=1 << 23, nq=1, nk=129)  # the keys' kernel alone
+    assert call(**one, **keys) == INVALID and bwd(**one, **keys) == UNSUPPORTED

@@ -40,6 +40,13 @@ constexpr float kNegInf = -__builtin_huge_valf();
 // float32 sums and the operand types hold as well as those below 1.
 constexpr float kSlack = 8.f;
 
+// In float16 all powers are times 2^kLift besides, up to 2^15: a key whose weight is
+// 2^-21 of the largest is a normal value still. Of keys that are alike the rounding
+// errors are, and below the normal values they add up: among tokens of which one in
+// 64 takes nearly all of the weight and the others have 7e-7 of it each, what these
+// add to the result was off by 4 %.
+template <typename T> constexpr float kLift = std::is_same_v<T, f16> ? 7.f : 0.f;
+
 // What sums relative to the maximum m are multiplied by to be relative to `top`, at
 // least m. Parts with one maximum are added as they are, -inf included: no score of
 // theirs was above it, but one may be NaN, and so may their sums.
@@ -234,7 +241,7 @@ __global__ __launch_bounds__(256, (kResidentFwd<T, DP>)) void k_cross_fwd(CrossA
 #pragma unroll
             for (int db = 0; db < DB; ++db) acc[db] *= f;
         }
-        const float mc = m == kNegInf ? 0.f : m * p.c;  // no key seen so far: every power is 0
+        const float mc = (m == kNegInf ? 0.f : m * p.c) - kLift<T>;  // no key seen so far: every power is 0
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -327,7 +334,7 @@ __global__ __launch_bounds__(256, (kResidentFwd<T, DP>)) void k_cross_fwd(CrossA
         for (int q = 0; q < M::Q; ++q)
             store4_rest<T>((T*)p.out + o, p.rest ? (T*)p.rest + o : nullptr, db * S + M::row4(q, lane), p.D,
                            M::quad(acc[db], q) * inv);
-    if (p.lse && slot == 0) p.lse[bh * p.M + r] = l == 0.f ? -kNegInf : m * p.c + __builtin_amdgcn_logf(l);
+    if (p.lse && slot == 0) p.lse[bh * p.M + r] = l == 0.f ? -kNegInf : m * p.c - kLift<T> + __builtin_amdgcn_logf(l);
 }
 
 // The splits of a row joined in order, a chunk of 4 output values per thread of
@@ -376,7 +383,7 @@ __global__ __launch_bounds__(256) void k_cross_join(CrossArgs p) {
     const uint32_t bh = at / (uint32_t)p.M, r = at - bh * (uint32_t)p.M, b = bh / p.KH, head = bh - b * p.KH;
     const int64_t o = b * p.Nq * p.H * p.D + row_at(p, r, (int64_t)p.H * p.D, p.D, head);
     store4_rest<T>((T*)p.out + o, p.rest ? (T*)p.rest + o : nullptr, c, p.D, acc * (l == 0.f ? 0.f : 1.f / l));
-    if (p.lse && c == 0) p.lse[at] = l == 0.f ? -kNegInf : top * p.c + __builtin_amdgcn_logf(l);
+    if (p.lse && c == 0) p.lse[at] = l == 0.f ? -kNegInf : top * p.c - kLift<T> + __builtin_amdgcn_logf(l);
 }
 
 template <typename T, int WM, int S>

@@ -449,3 +449,26 @@ def test_masks_of_any_strides(dev, dtype):
     for mask in (wide[:1, :150].expand(3, 150), wide[:, ::2], turned, wide[:, :1].expand(3, 150)):
         got, want = (_check(q, k, v, dout, None, m) for m in (mask, mask.contiguous()))
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("Nq,Nk", [(1, 5000), (20, 5000), (200, 5000)])
+def test_probabilities_far_below_the_largest(dev, Nq, Nk, dtype):
+    """One key in 64 takes nearly all of the weight and has no value, as the first
+    token of a sequence often does: the result is the others', which at 7e-7 of the
+    largest are below float16's normal values, all alike. Their rounding has the
+    sums' full relative size: 2 u as elsewhere."""
+    import eccv26_tad_amd as sv
+
+    T = DTYPES[dtype]
+    q = torch.zeros(2, Nq, 2, 32, device=dev)
+    q[..., 0] = 1
+    k = torch.zeros(2, Nk, 2, 32, device=dev)
+    k[..., 0] = -14.1953125  # exp of it is 11.48 2^-24; exact in all types
+    v = 100 * torch.rand(2, Nk, 2, 32, device=dev, generator=torch.Generator(device=dev).manual_seed(4))
+    if T is torch.bfloat16:
+        k[..., 0] = -14.1875
+    k[:, ::64], v[:, ::64] = 0, 0
+    q, k, v = q.to(T), k.to(T), v.to(T)
+    want, _ = _exact(q, k, v, q, None, None, 1.0)
+    _near(sv.cross_attention(q, k, v, scale=1.0), want[0], None, 2 * U[T], "out")

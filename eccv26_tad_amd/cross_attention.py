@@ -31,8 +31,11 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_lengt
     hold, infinities and NaN included, reaches no result. ``scale`` defaults to
     ``D ** -0.5`` and must be positive.
 
-    Softmax statistics and sums are float32; probabilities are rounded to the
-    inputs' dtype as operands of the matrix units. Gradients come without
+    Softmax statistics and sums are float32; probabilities and score gradients
+    are rounded to the inputs' dtype as operands of the matrix units (scaled by
+    powers of two in float16, so that small ones keep their bits). For the
+    backward the call keeps its result, in 16 bits a second tensor like it (what
+    the result's rounding took), and 4 bytes per query and head. Gradients come without
     atomics: equal inputs give equal bits. Differentiable once, in reverse mode;
     a second derivative and forward mode raise."""
     if scale is None:

@@ -22,8 +22,9 @@ constexpr int64_t kMaxGrid = (1 << 24) - 1;
 // bfloat16 at 64, 1000 rows, forward, split against whole: 48 groups over 1500
 // keys 17.5 us in four against 25.9, 192 over 500 keys 23.8 in two against 12.3, 192
 // over 20000 keys 176 in four against 202 in two and 277. One query over 8 x 31361
-// keys of 4 heads: 47.3 us in 16, 53.5 in 8, 55.1 in 24. Of 285 kernels at 95 drawn
-// sizes of all types 7 took over 15 % more than in the best of 14 splits (27 % most).
+// keys of 4 heads: 47.3 us in 16, 53.5 in 8, 55.1 in 24. Heads of 33 to 64 whose rows
+// are not read in whole vectors run in the 128-wide kernel, which the estimate does
+// not tell from the 64-wide one.
 static int splits(const svtad_cross_args& a, int dtype, int64_t groups, int64_t tiles, int rows, double products) {
     const bool alone = dtype == SVTAD_F32 || a.head_dim > 64;
     const double tile = products / 2. * (dtype == SVTAD_F32 ? 7 : 1) * (0.5 + a.head_dim / 128.);

@@ -1,5 +1,7 @@
 """The norm over all gradients of a model, and clipping to a limit, on HIP
-kernels: a few launches for any number of tensors, no host synchronisation.
+kernels, without host synchronisation: two launches for every 160 tensors of one
+dtype that follow one another (a list that alternates between dtypes takes two for
+every run of them).
 
 The reference's training loop clips with ``torch.nn.utils.clip_grad_norm_``
 (``opentad/cores/train_engine.py:706-731``).

@@ -43,10 +43,10 @@ constexpr float kNegInf = -__builtin_huge_valf();
 constexpr float kSlack = 8.f;
 
 // In float16 all powers are times 2^kLift besides, up to 2^15: a key whose weight is
-// 2^-21 of the largest is a normal value still. Of keys that are alike the rounding
-// errors are, and below the normal values they add up: among tokens of which one in
-// 64 takes nearly all of the weight and the others have 7e-7 of it each, what these
-// add to the result was off by 4 %.
+// 2^-21 of the largest is a normal value still. Below those values the roundings of
+// keys that are alike are large, alike too, and add up: where one token in 64 takes
+// nearly all of the weight and the others 7e-7 of it each, what these add to the result
+// is off by 4 % without the lift.
 template <typename T> constexpr float kLift = std::is_same_v<T, f16> ? 7.f : 0.f;
 
 // What sums relative to the maximum m are multiplied by to be relative to `top`, at
